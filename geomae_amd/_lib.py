@@ -44,6 +44,15 @@ class GeomaeSstStackLayout(ctypes.Structure):
                 ("num_fbundles", c_void_p), ("fitems", c_void_p), ("num_fitems", c_void_p)]
 
 
+class GeomaeAdamwTensor(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("param", "exp_avg", "exp_avg_sq", "exp_avg_exponent", "exp_avg_sq_exponent", "master",
+                                         "step")] + [("numel", c_int64), ("dtype", c_int32), ("index", c_int32)])
+
+
+class GeomaeAdamwHyper(ctypes.Structure):
+    _fields_ = [(n, c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [("lr_ptr", c_void_p)]
+
+
 class GeomaeVfeArgs(ctypes.Structure):
     _fields_ = [("feat_sorted", c_void_p), ("pid_sorted", c_void_p), ("seg_start", c_void_p), ("num_points", c_int64),
                 ("max_pillars", c_int32), ("w0", c_void_p), ("w1", c_void_p), ("scale0", c_void_p), ("shift0", c_void_p),
@@ -205,6 +214,11 @@ SIGNATURES = {
     "geomae_grad_sumsq": (ctypes.c_int, [P, c_int64, P, P]),
     "geomae_adamw_step": (ctypes.c_int, [P, P, P, P, c_int64, c_int64, c_float, c_float, c_float, c_float, c_float,
                                          c_int64, c_float, P, c_float, c_int32, P, c_int64, c_int64, P, P]),
+    "geomae_multi_adamw_chunk": (c_int32, []),
+    "geomae_multi_adamw_workspace_bytes": (c_int64, [c_int32]),
+    "geomae_multi_adamw_step": (ctypes.c_int, [P, P, P, c_int32, P, P, P, c_int32, c_int32, c_double, c_double, P, c_int32,
+                                               ctypes.c_uint32, P, P, c_int64, P]),
+    "geomae_adamw_moments8": (ctypes.c_int, [P, P, P, P, c_int64, P, P, P]),
     "geomae_bn_finalize": (ctypes.c_int, [P, c_double, P, c_int32, P, P, c_float, c_float, c_int32, P, P, P, P, P, P, P, P]),
     "geomae_vfe_stats0": (ctypes.c_int, [POINTER(GeomaeVfeArgs), P, P]),
     "geomae_vfe_layer0": (ctypes.c_int, [POINTER(GeomaeVfeArgs), P, P, P]),

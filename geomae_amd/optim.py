@@ -1,0 +1,333 @@
+"""AdamW over many tensors where they lie: `MultiTensorAdamW`, a torch optimizer on the HIP kernels of csrc/multi_adamw.hip.
+
+`train.FlatAdamW` updates ONE flat fp32 buffer that every parameter was re-homed into.  This one takes the parameters as they
+are -- fp32, bf16 or fp16, frozen ones among them, convolution weights in channels_last, optionally with fp32 masters behind
+16-bit weights -- and holds their moments in 32 or in 8 bits.  A step is a norm pass (where a norm is wanted), one small launch
+for the per-tensor scalars and one update launch for up to 256 tensors each, whatever the tensors' sizes; step counts live on
+the device, so a captured step goes on counting when it is replayed."""
+import ctypes
+
+import torch
+
+from . import _lib
+from .ops import _ptr
+
+BLOCK = 32                      # elements that share an exponent byte (8-bit moments); tensors start at multiples of it
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ZERO_EXPONENT = 16             # exponent byte of a block of zeros
+
+
+def _dense(t):
+    """Non-overlapping and dense in some order of its dimensions (contiguous, channels_last, a transpose of either)."""
+    if t.numel() == 0:
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+class MultiTensorAdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's update (decoupled weight decay) of all parameters in two or three launches per 256 tensors.
+
+    params: tensors or parameter groups (lr, betas, eps, weight_decay per group); all on one GPU, each dense (in any order of
+    its dimensions), float32 / bfloat16 / float16.  A group's lr may be a 0-d float32 tensor on that GPU: a captured step then
+    reads it at every replay.
+    state_bits: 32 = moments in fp32; 8 = one byte per moment and element plus one exponent byte for 32 elements, rounded
+    stochastically (reproducibly: a function of seed, parameter index, step and element).  The second moment is held as its root.
+    master_weights: keep an fp32 copy of every 16-bit parameter and update that; the parameter is its rounding.  Without
+    it a 16-bit parameter is updated in place and rounded to nearest, as torch.optim.AdamW does.
+
+    The defaults are the pre-training config's (lr 1e-5, weight_decay 0.05).  Gradients are read where they are when step() is
+    called; parameters without one are skipped and do not count the step."""
+
+    def __init__(self, params, lr=1e-5, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.05, state_bits=32, master_weights=False,
+                 seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
+        self._check_hyper(dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.master_weights, self.seed = int(state_bits), bool(master_weights), int(seed)
+        if not 0 <= self.seed < 2 ** 32:
+            raise ValueError("seed must be in [0, 2**32)")
+        self._arena, self._table, self._building = None, None, True
+        self.grad_norm = None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self._building = False
+        self._build()
+
+    # ------------------------------------------------------------------------------------------------ construction
+    @staticmethod
+    def _check_hyper(g):
+        b1, b2 = g["betas"]
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"betas must be in [0, 1), got {g['betas']}")
+        if g["eps"] < 0.0 or g["weight_decay"] < 0.0 or (not torch.is_tensor(g["lr"]) and g["lr"] < 0.0):
+            raise ValueError(f"lr, eps and weight_decay must not be negative, got {g['lr']}, {g['eps']}, {g['weight_decay']}")
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        try:
+            self._check_hyper(g)
+            if torch.is_tensor(g["lr"]) and (g["lr"].dtype != torch.float32 or g["lr"].numel() != 1 or not g["lr"].is_cuda):
+                raise ValueError("a tensor lr must be one float32 value on the GPU")
+            self._check_params(g["params"])
+        except Exception:
+            self.param_groups.pop()
+            raise
+        if not self._building:
+            self._build()
+
+    def _check_params(self, params):
+        first = self.param_groups[0]["params"][0]
+        if len({id(p) for p in params}) != len(params):
+            raise ValueError("MultiTensorAdamW: a parameter is listed twice")
+        for p in params:
+            if not p.is_cuda:
+                raise RuntimeError("MultiTensorAdamW: parameters must be CUDA tensors (geomae_amd has no CPU path)")
+            if p.device != first.device:
+                raise RuntimeError(f"MultiTensorAdamW: parameters on {first.device} and on {p.device}: one optimizer per GPU")
+            if p.dtype not in _DTYPE:
+                raise RuntimeError(f"MultiTensorAdamW: parameters must be float32, bfloat16 or float16, got {p.dtype}")
+            if p.layout != torch.strided or not _dense(p):
+                raise RuntimeError("MultiTensorAdamW: parameters must be dense (no gaps or overlaps between their elements)")
+
+    def _params(self):
+        return [p for g in self.param_groups for p in g["params"]]
+
+    def _build(self):
+        """Moments of all parameters in one arena per kind, each parameter's part starting at a multiple of 32 elements; a
+        parameter's state tensors are views of it in the parameter's own layout.  Parameters that were there keep theirs."""
+        params, old = self._params(), self._arena
+        dev = params[0].device
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("MultiTensorAdamW: two parameters share memory")
+        offsets, total = [], 0
+        for p in params:
+            offsets.append(total)
+            total += -(-p.numel() // BLOCK) * BLOCK
+        kind = torch.float32 if self.state_bits == 32 else torch.uint8
+        arena = {"exp_avg": torch.zeros(total, dtype=kind, device=dev), "exp_avg_sq": torch.zeros(total, dtype=kind, device=dev),
+                 "step": torch.zeros(len(params), dtype=torch.int64, device=dev)}
+        if self.state_bits == 8:
+            for k in ("exp_avg_exponent", "exp_avg_sq_exponent"):
+                arena[k] = torch.full((total // BLOCK,), _ZERO_EXPONENT, dtype=torch.uint8, device=dev)
+        if self.master_weights:
+            arena["master"] = torch.zeros(total, dtype=torch.float32, device=dev)
+        self._arena, self.offsets = arena, offsets
+        for i, (p, off) in enumerate(zip(params, offsets)):
+            had = self.state.get(p) if old is not None else None
+            new = self._views(arena, i, p, off)
+            for k, v in new.items():
+                if had:
+                    v.copy_(had[k])
+                elif k == "master":
+                    v.copy_(p.detach())
+            self.state[p] = new
+        lib = _lib.load()
+        chunk = lib.geomae_multi_adamw_chunk()
+        counts = [-(-p.numel() // chunk) for p in params]
+        first = [0]
+        for c in counts:
+            first.append(first[-1] + c)
+        tensor = torch.repeat_interleave(torch.arange(len(params), dtype=torch.int32), torch.tensor(counts, dtype=torch.int64))
+        within = torch.arange(first[-1], dtype=torch.int64) - torch.tensor(first[:-1], dtype=torch.int64)[tensor.long()]
+        self._chunks = torch.stack([tensor, within.int()], 1).contiguous().to(dev)
+        n = len(params)
+        self._first_chunk = (ctypes.c_int64 * (n + 1))(*first)
+        self._grad_ptrs, self._hyper_of = (ctypes.c_void_p * n)(), (ctypes.c_int32 * n)()
+        ws = lib.geomae_multi_adamw_workspace_bytes(n)
+        self._workspace = torch.empty(ws, dtype=torch.uint8, device=dev)
+        self._norm_word = torch.zeros((), dtype=torch.float32, device=dev)
+        self._fill_table()
+
+    @staticmethod
+    def _part(flat, off, p):
+        """p's own part of an arena, in p's layout."""
+        return flat.as_strided(p.shape, p.stride(), off) if p.numel() else flat[off:off].view(p.shape)
+
+    def _views(self, arena, i, p, off):
+        blocks = slice(off // BLOCK, off // BLOCK + -(-p.numel() // BLOCK))
+        out = {"step": arena["step"][i]}
+        for k in ("exp_avg", "exp_avg_sq"):
+            out[k] = self._part(arena[k], off, p)
+            if self.state_bits == 8:
+                out[k + "_exponent"] = arena[k + "_exponent"][blocks]
+        if self.master_weights and p.dtype != torch.float32:
+            out["master"] = self._part(arena["master"], off, p)
+        return out
+
+    def _fill_table(self):
+        """The device table of addresses.  A table that a captured step may still read is kept as long as this optimizer."""
+        params, a, rows = self._params(), self._arena, None
+        rows = (_lib.GeomaeAdamwTensor * len(params))()
+        for i, (p, off) in enumerate(zip(params, self.offsets)):
+            r = rows[i]
+            item = a["exp_avg"].element_size()
+            r.param = p.data_ptr()
+            r.exp_avg, r.exp_avg_sq = a["exp_avg"].data_ptr() + off * item, a["exp_avg_sq"].data_ptr() + off * item
+            if self.state_bits == 8:
+                r.exp_avg_exponent = a["exp_avg_exponent"].data_ptr() + off // BLOCK
+                r.exp_avg_sq_exponent = a["exp_avg_sq_exponent"].data_ptr() + off // BLOCK
+            r.master = a["master"].data_ptr() + 4 * off if self.master_weights and p.dtype != torch.float32 else None
+            r.step = a["step"].data_ptr() + 8 * i
+            r.numel, r.dtype, r.index = p.numel(), _DTYPE[p.dtype], i
+        host = torch.frombuffer(bytearray(rows), dtype=torch.uint8)
+        self._retired = getattr(self, "_retired", []) + ([self._table] if self._table is not None else [])
+        self._table = host.to(params[0].device)
+        self._where = [p.data_ptr() for p in params]
+        self._layout = [(p.shape, p.stride(), p.dtype) for p in params]
+
+    # ------------------------------------------------------------------------------------------------ the step
+    @torch.no_grad()
+    def step(self, closure=None, max_norm=0.0, grad_scale=1.0, skip_nonfinite=False):
+        """One update of every parameter that has a gradient.  max_norm > 0 clips the gradients to that norm over all of
+        them (torch.nn.utils.clip_grad_norm_); grad_scale (a number, or one float32 value on the GPU) multiplies them first;
+        skip_nonfinite leaves everything as it was if their norm is not finite.  After a step with max_norm or
+        skip_nonfinite, `grad_norm` is the scaled gradients' norm before clipping (a 0-d tensor that the next step
+        overwrites).  Gradients are not changed."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params = self._params()
+        dev = params[0].device
+        where = [p.data_ptr() for p in params]
+        if where != self._where:
+            if [(p.shape, p.stride(), p.dtype) for p in params] != self._layout:
+                raise RuntimeError("MultiTensorAdamW: a parameter changed its shape, layout or dtype; make a new optimizer")
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("MultiTensorAdamW: a parameter's storage moved; take one step outside the capture first")
+            self._check_params(params)
+            self._fill_table()
+        keep, i = [], 0
+        hypers, number = [], {}
+        for group in self.param_groups:
+            lr = group["lr"]
+            key = (lr.data_ptr() if torch.is_tensor(lr) else float(lr), torch.is_tensor(lr), *map(float, group["betas"]),
+                   float(group["eps"]), float(group["weight_decay"]))
+            k = number.get(key)
+            if k is None:
+                self._check_hyper(group)
+                k = number[key] = len(hypers)
+                hypers.append(key)
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    self._grad_ptrs[i] = None
+                else:
+                    if g.stride() != p.stride() or g.dtype != p.dtype or g.layout != torch.strided or g.device != dev:
+                        g = self._like(g, p)
+                        keep.append(g)
+                    self._grad_ptrs[i] = g.data_ptr()
+                    self._hyper_of[i] = k
+                i += 1
+        hyper_rows = (_lib.GeomaeAdamwHyper * max(1, len(hypers)))()
+        for row, (lr, is_tensor, b1, b2, eps, wd) in zip(hyper_rows, hypers):
+            row.lr, row.lr_ptr = (0.0, lr) if is_tensor else (lr, None)
+            row.beta1, row.beta2, row.eps, row.weight_decay = b1, b2, eps, wd
+        scale_ptr, scale = None, 1.0
+        if torch.is_tensor(grad_scale):
+            if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev:
+                raise RuntimeError("MultiTensorAdamW: a tensor grad_scale must be one float32 value on the parameters' GPU")
+            scale_ptr = grad_scale.data_ptr()
+        else:
+            scale = float(grad_scale)
+        wants_norm = float(max_norm or 0.0) > 0.0 or skip_nonfinite
+        with torch.cuda.device(dev):
+            stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+            _lib.check(_lib.load().geomae_multi_adamw_step(
+                _ptr(self._table), _ptr(self._chunks), self._first_chunk, len(params), self._grad_ptrs, self._hyper_of,
+                ctypes.addressof(hyper_rows), len(hypers), self.state_bits, float(max_norm or 0.0), scale, scale_ptr,
+                int(bool(skip_nonfinite)), self.seed, _ptr(self._norm_word) if wants_norm else None, _ptr(self._workspace),
+                self._workspace.numel(), stream), "geomae_multi_adamw_step")
+        if wants_norm:
+            self.grad_norm = self._norm_word
+        return loss
+
+    @staticmethod
+    def _like(g, p):
+        """A gradient in another layout than its parameter's, as a copy in the parameter's."""
+        if g.layout != torch.strided:
+            raise RuntimeError("MultiTensorAdamW: sparse gradients are not supported")
+        if g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
+            raise RuntimeError(f"MultiTensorAdamW: a gradient ({g.dtype}, {tuple(g.shape)}, {g.device}) does not match its parameter "
+                               f"({p.dtype}, {tuple(p.shape)}, {p.device})")
+        return torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
+
+    # ------------------------------------------------------------------------------------------------ state
+    def moments(self):
+        """(first, second moment) of all parameters as two flat tensors, parameter i's from self.offsets[i] on in its memory
+        order.  32 bits: the fp32 moments themselves (not a copy).  8 bits: the values that the codes stand for, in bfloat16
+        (which holds them exactly), the second as the root that is stored."""
+        a = self._arena
+        if self.state_bits == 32:
+            return a["exp_avg"], a["exp_avg_sq"]
+        n, dev = a["exp_avg"].numel(), a["exp_avg"].device
+        out = [torch.empty(n, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+        with torch.cuda.device(dev):
+            _lib.check(_lib.load().geomae_adamw_moments8(
+                _ptr(a["exp_avg"]), _ptr(a["exp_avg_exponent"]), _ptr(a["exp_avg_sq"]), _ptr(a["exp_avg_sq_exponent"]), n,
+                _ptr(out[0]), _ptr(out[1]), ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), "geomae_adamw_moments8")
+        return out[0], out[1]
+
+    def masters(self):
+        """The fp32 masters as one flat tensor (not a copy), parameter i's from self.offsets[i] on; fp32 parameters have none."""
+        if not self.master_weights:
+            raise RuntimeError("MultiTensorAdamW: made without master_weights")
+        return self._arena["master"]
+
+    def load_flat_state(self, state, step):
+        """Fill the moments (and masters) from flat tensors laid out as moments() and masters() give them -- at 8 bits the codes
+        and their exponent bytes -- and set every parameter's step count."""
+        if set(state) != set(self._arena) - {"step"}:
+            raise ValueError(f"flat state must have {sorted(set(self._arena) - {'step'})}, got {sorted(state)}")
+        for k, v in state.items():
+            if v.shape != self._arena[k].shape or v.dtype != self._arena[k].dtype:
+                raise ValueError(f"flat state {k}: {tuple(v.shape)} {v.dtype}, expected {tuple(self._arena[k].shape)} {self._arena[k].dtype}")
+        for k, v in state.items():
+            self._arena[k].copy_(v)
+        self._arena["step"].fill_(int(step))
+
+    def state_dict(self):
+        sd = super().state_dict()
+        sd["state_bits"], sd["master_weights"], sd["seed"] = self.state_bits, self.master_weights, self.seed
+        return sd
+
+    @torch.no_grad()
+    def load_state_dict(self, sd):
+        """A state_dict of this class with the same state_bits and masters, or (32 bits) one of torch.optim.AdamW; masters
+        that it does not hold are taken from the parameters."""
+        if int(sd.get("state_bits", 32)) != self.state_bits:
+            raise ValueError(f"the state holds moments in {sd.get('state_bits', 32)} bits, this optimizer in {self.state_bits}")
+        groups = sd["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("the state's parameter groups do not match this optimizer's")
+        if any(g.get("amsgrad") or g.get("maximize") for g in groups):
+            raise ValueError("amsgrad and maximize are not supported")
+        params, ids = self._params(), [i for g in groups for i in g["params"]]
+        todo = []
+        for p, i in zip(params, ids):
+            st, mine = sd["state"].get(i), self.state[p]
+            if st is None:
+                continue
+            for k, v in mine.items():
+                if k == "master" and k not in st:
+                    todo.append((v, p.detach()))
+                    continue
+                if k not in st:
+                    raise ValueError(f"the state of parameter {i} has no {k}")
+                x = st[k] if torch.is_tensor(st[k]) else torch.tensor(st[k])
+                if k != "step" and (x.shape != v.shape or (x.dtype == torch.uint8) != (v.dtype == torch.uint8)):
+                    raise ValueError(f"the state of parameter {i}: {k} is {tuple(x.shape)} {x.dtype}, expected {tuple(v.shape)} {v.dtype}")
+                todo.append((v, x.reshape(v.shape)))
+        for g, h in zip(self.param_groups, groups):
+            self._check_hyper({**g, **{k: v for k, v in h.items() if k != "params"}})
+        for v, x in todo:
+            v.copy_(x)
+        for g, h in zip(self.param_groups, groups):
+            g.update({k: v for k, v in h.items() if k != "params"})
+        self.seed = int(sd.get("seed", self.seed))

@@ -769,6 +769,55 @@ int geomae_adamw_step(float* params, float* grads, float* exp_avg, float* exp_av
                       float* grad_norm_out, int64_t no_decay2_start, int64_t no_decay2_count, double* zero_after,
                       geomaeStream_t stream);
 
+/* ------------------------------------------------------------------ AdamW over many tensors
+ * The same update for parameters that stay where they are, each an own dense tensor of fp32, bf16 or fp16 with a gradient
+ * of its own type and layout, moments in fp32 or in 8 bits, optionally with fp32 masters behind 16-bit parameters.
+ *
+ * GeomaeAdamwTensor: one row per tensor of a DEVICE table that stands for as long as the tensors do.  `numel` elements are
+ * taken in memory order.  exp_avg, exp_avg_sq and master are zero-padded to a multiple of 32 elements and aligned to 16
+ * bytes; param and the gradient need no more than their element's alignment.  step (device) counts the steps this tensor
+ * has taken; the call advances it.  index: the tensor's number in the hash of the 8-bit rounding.
+ * 8-bit moments: exp_avg codes (sign, 4 exponent and 3 fraction bits) and exp_avg_sq codes (the ROOT of the second moment:
+ * 4 + 4 bits, no sign), one byte per element; *_exponent one byte E for every 32 elements (16 .. 254; 16 where the block is
+ * zero): value = code value * 2^(E - 135).  Rounding is stochastic, a function of (seed, index, step, element) alone.
+ *
+ * geomae_multi_adamw_step: chunks (device) [first_chunk[num_tensors]][2] = (tensor, chunk of that tensor), a chunk being
+ * geomae_multi_adamw_chunk() elements; first_chunk (host) [num_tensors + 1].  grads (host) [num_tensors]: device addresses,
+ * NULL = the tensor has no gradient and is left as it is, its step too.  hyper_of (host) [num_tensors] indexes hypers (host)
+ * [num_hypers]; lr_ptr (device, or NULL) replaces lr.  Gradients are scaled by grad_scale * (grad_scale_ptr ?
+ * *grad_scale_ptr : 1) and, max_norm > 0, clipped to that norm over ALL tensors, whose pre-clip value grad_norm_out (device,
+ * or NULL) receives.  skip_nonfinite != 0: a norm that is not finite leaves every parameter, moment and step as it was.
+ * The arguments are read before the call returns; the launches can be captured (gradients and lr_ptr at the same addresses). */
+enum { GEOMAE_DTYPE_F32 = 0, GEOMAE_DTYPE_BF16 = 1, GEOMAE_DTYPE_F16 = 2 };
+typedef struct GeomaeAdamwTensor {
+    void* param;
+    void* exp_avg;
+    void* exp_avg_sq;
+    uint8_t* exp_avg_exponent;       /* 8-bit moments only */
+    uint8_t* exp_avg_sq_exponent;
+    float* master;                   /* or NULL: the parameter itself is updated */
+    int64_t* step;
+    int64_t numel;
+    int32_t dtype;                   /* GEOMAE_DTYPE_* of param and gradient */
+    int32_t index;
+} GeomaeAdamwTensor;
+typedef struct GeomaeAdamwHyper {
+    double lr, beta1, beta2, eps, weight_decay;
+    const float* lr_ptr;
+} GeomaeAdamwHyper;
+int32_t geomae_multi_adamw_chunk(void);
+int64_t geomae_multi_adamw_workspace_bytes(int32_t num_tensors);
+int geomae_multi_adamw_step(const GeomaeAdamwTensor* table, const int32_t* chunks, const int64_t* first_chunk, int32_t num_tensors,
+                            const void* const* grads, const int32_t* hyper_of, const GeomaeAdamwHyper* hypers,
+                            int32_t num_hypers, int32_t state_bits, double max_norm, double grad_scale,
+                            const float* grad_scale_ptr, int32_t skip_nonfinite, uint32_t seed, float* grad_norm_out,
+                            void* workspace, int64_t workspace_bytes, geomaeStream_t stream);
+/* 8-bit moments of num_elems elements (a multiple of 32) as the values they stand for: exp_avg and the root of exp_avg_sq in
+ * bf16, which holds every one of them exactly */
+int geomae_adamw_moments8(const uint8_t* exp_avg, const uint8_t* exp_avg_exponent, const uint8_t* exp_avg_sq,
+                          const uint8_t* exp_avg_sq_exponent, int64_t num_elems, void* exp_avg_out, void* root_out,
+                          geomaeStream_t stream);
+
 /* BatchNorm parameter gradients from the LOCAL backward sums of the fused VFE (naiveSyncBN1d at world > 1: they are
  * added before the sums are all-reduced for the input gradient): d_beta[c] += bsums[c], d_gamma[c] += bsums[C + c]. */
 int geomae_bn_param_grad_add(const double* bsums /*[2C]*/, int32_t channels, float* d_beta, float* d_gamma,
