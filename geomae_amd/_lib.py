@@ -219,6 +219,11 @@ SIGNATURES = {
     "geomae_multi_adamw_step": (ctypes.c_int, [P, P, P, c_int32, P, P, P, c_int32, c_int32, c_double, c_double, P, c_int32,
                                                ctypes.c_uint32, P, P, c_int64, P]),
     "geomae_adamw_moments8": (ctypes.c_int, [P, P, P, P, c_int64, P, P, P]),
+    "geomae_group_norm_workspace_bytes": (c_int64, [c_int32, c_int64, c_int32, c_int32, c_int32, c_int32]),
+    "geomae_group_norm_forward": (ctypes.c_int, [P, c_int32, c_int32, c_int64, c_int32, c_int32, P, P, c_int32, c_double, c_int32, P, P,
+                                                 P, c_int64, P]),
+    "geomae_group_norm_backward": (ctypes.c_int, [P, P, c_int32, c_int32, c_int64, c_int32, c_int32, P, P, c_int32, c_int32, P, P, P, P,
+                                                  P, c_int64, P]),
     "geomae_bn_finalize": (ctypes.c_int, [P, c_double, P, c_int32, P, P, c_float, c_float, c_int32, P, P, P, P, P, P, P, P]),
     "geomae_vfe_stats0": (ctypes.c_int, [POINTER(GeomaeVfeArgs), P, P]),
     "geomae_vfe_layer0": (ctypes.c_int, [POINTER(GeomaeVfeArgs), P, P, P]),

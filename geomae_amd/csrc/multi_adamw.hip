@@ -226,7 +226,7 @@ __global__ __launch_bounds__(kMaThreads) void multi_prepare_kernel(MaPrepareArgs
         if (a.want_norm) {
             const float norm = (float)(sqrt(red[0] + red[1] + red[2] + red[3]) * fabs((double)scale));
             if (a.grad_norm) *a.grad_norm = norm;
-            if (a.max_norm > 0.0) {
+            if (a.max_norm > 0.0 && a.max_norm < INFINITY) {
                 const float c = (float)a.max_norm / (norm + 1e-6f);
                 coef *= c > 1.0f ? 1.0f : c;                         // NaN stays NaN
             }

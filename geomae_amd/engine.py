@@ -26,7 +26,8 @@ def supported(model):
     """The engine covers exactly the configuration the fused kernels cover (the mae_sst config)."""
     bb, ve = getattr(model, "backbone", None), getattr(model, "voxel_encoder", None)
     return (bb is not None and ve is not None and getattr(bb, "fused", False) and getattr(ve, "use_fused", True)
-            and hasattr(model, "_tcfg") and len(ve.vfe_layers) == 2 and next(model.parameters()).is_cuda)
+            and hasattr(model, "_tcfg") and len(ve.vfe_layers) == 2
+            and all(isinstance(l.norm, torch.nn.BatchNorm1d) for l in ve.vfe_layers) and next(model.parameters()).is_cuda)
 
 
 class PretrainEngine:

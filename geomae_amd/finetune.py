@@ -18,7 +18,8 @@ import torch
 from torch import nn
 
 from . import ops
-from .registry import BACKBONES, DETECTORS, MIDDLE_ENCODERS, NECKS, MODELS, build_norm_layer
+from .norm import build_norm_relu
+from .registry import BACKBONES, DETECTORS, MIDDLE_ENCODERS, NECKS, MODELS
 from .sst import BasicShiftBlock, PackedLayers, _FusedStack, pos_embed_table
 
 
@@ -103,10 +104,10 @@ class SSTSecondPretrainedv1(nn.Module):
         blocks = []
         for i, layer_num in enumerate(layer_nums):
             mods = [nn.Conv2d(in_filters[i], conv_out_channels[i], 3, stride=layer_strides[i], padding=1, bias=bias),
-                    build_norm_layer(norm_cfg, conv_out_channels[i])[1], nn.ReLU(inplace=True)]
+                    *build_norm_relu(norm_cfg, conv_out_channels[i])]
             for _ in range(layer_num):
                 mods += [nn.Conv2d(conv_out_channels[i], conv_out_channels[i], 3, padding=1, bias=bias),
-                         build_norm_layer(norm_cfg, conv_out_channels[i])[1], nn.ReLU(inplace=True)]
+                         *build_norm_relu(norm_cfg, conv_out_channels[i])]
             blocks.append(nn.Sequential(*mods))
         self.conv_blocks = nn.ModuleList(blocks)
         self.register_buffer("pos_table", pos_embed_table(self.window_shape, d_model[0], pos_temperature), persistent=False)
@@ -164,7 +165,7 @@ class SECONDFPN(nn.Module):
             else:
                 k = int(np.round(1 / stride))
                 up = nn.Conv2d(in_channels[i], oc, kernel_size=k, stride=k, bias=bool(conv_cfg.get("bias", False)))
-            deblocks.append(nn.Sequential(up, build_norm_layer(norm_cfg, oc)[1], nn.ReLU(inplace=True)))
+            deblocks.append(nn.Sequential(up, *build_norm_relu(norm_cfg, oc)))
         self.deblocks = nn.ModuleList(deblocks)
         for m in self.modules():                                  # init_cfg: Kaiming for the deconvs, BN weight 1
             if isinstance(m, nn.ConvTranspose2d):

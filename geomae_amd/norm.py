@@ -19,7 +19,7 @@ import torch
 from torch import distributed as dist
 from torch import nn
 
-from .registry import NORM_LAYERS
+from .registry import NORM_LAYERS, build_norm_layer
 
 
 def _cross_rank_active(module):
@@ -96,5 +96,43 @@ class NaiveSyncBatchNorm2d(_CrossRankMixin, nn.BatchNorm2d):
     """[N, C, H, W] activations: the fine-tune backbone's conv stack and SECONDFPN (mmdet3d/ops/norm.py:89-140)."""
 
 
+class GroupNormAct(nn.Module):
+    """Group norm of [N, C, *] activations with an optional activation in the same pass (ops.group_norm_act): the 'GN' of a
+    norm_cfg, e.g. dict(type='GN', num_groups=32).  Statistics are a sample's own: no running averages, nothing exchanged
+    between ranks, the same in training and evaluation.  Parameters are named as in nn.GroupNorm.  Activations that are not
+    in channels-last memory are copied into it; the output is in channels-last memory."""
+
+    def __init__(self, num_channels, num_groups, eps=1e-5, affine=True, activation=None):
+        super().__init__()
+        if num_groups < 1 or num_channels % num_groups:
+            raise ValueError(f"{num_channels} channels do not divide into {num_groups} groups")
+        self.num_channels, self.num_groups, self.eps, self.affine, self.activation = num_channels, num_groups, eps, affine, activation
+        if affine:
+            self.weight, self.bias = nn.Parameter(torch.ones(num_channels)), nn.Parameter(torch.zeros(num_channels))
+        else:
+            self.register_parameter("weight", None)
+            self.register_parameter("bias", None)
+
+    def forward(self, input):
+        from . import ops
+        if input.is_cuda and input.dim() >= 2 and not ops._channels_last(input):
+            input = ops._to_channels_last(input)
+        return ops.group_norm_act(input, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+
+    def extra_repr(self):
+        return f"{self.num_groups}, {self.num_channels}, eps={self.eps}, affine={self.affine}, activation={self.activation}"
+
+
+NORM_LAYERS.register_module("GN", module=GroupNormAct)
 NORM_LAYERS.register_module("BN1d", module=nn.BatchNorm1d)
 NORM_LAYERS.register_module(["BN", "BN2d"], module=nn.BatchNorm2d)
+
+
+def build_norm_relu(cfg, num_features):
+    """[norm, ReLU] of a conv stage.  A group norm takes the ReLU (or the activation that its cfg names) into its own pass; the
+    module in the ReLU's place keeps the numbering of the stage's parameters in a state_dict."""
+    norm = build_norm_layer(cfg, num_features)[1]
+    if isinstance(norm, GroupNormAct):
+        norm.activation = norm.activation or "relu"
+        return [norm, nn.Identity()]
+    return [norm, nn.ReLU(inplace=True)]

@@ -185,7 +185,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, closure=None, max_norm=0.0, grad_scale=1.0, skip_nonfinite=False):
         """One update of every parameter that has a gradient.  max_norm > 0 clips the gradients to that norm over all of
-        them (torch.nn.utils.clip_grad_norm_); grad_scale (a number, or one float32 value on the GPU) multiplies them first;
+        them (torch.nn.utils.clip_grad_norm_; infinity: only the norm is wanted); grad_scale (a number, or one float32 value on the GPU) multiplies them first;
         skip_nonfinite leaves everything as it was if their norm is not finite.  After a step with max_norm or
         skip_nonfinite, `grad_norm` is the scaled gradients' norm before clipping (a 0-d tensor that the next step
         overwrites).  Gradients are not changed."""
@@ -244,6 +244,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                 ctypes.addressof(hyper_rows), len(hypers), self.state_bits, float(max_norm or 0.0), scale, scale_ptr,
                 int(bool(skip_nonfinite)), self.seed, _ptr(self._norm_word) if wants_norm else None, _ptr(self._workspace),
                 self._workspace.numel(), stream), "geomae_multi_adamw_step")
+        torch.autograd.graph.increment_version(params)
         if wants_norm:
             self.grad_norm = self._norm_word
         return loss

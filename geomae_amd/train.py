@@ -396,7 +396,8 @@ class Trainer:
     def __init__(self, model, optimizer_cfg=None, grad_clip=None, lr_schedule=None):
         from .configs import GRAD_CLIP, OPTIMIZER
         ocfg = dict(optimizer_cfg or OPTIMIZER)
-        assert ocfg.pop("type") == "AdamW"
+        otype = ocfg.pop("type")
+        assert otype in ("AdamW", "MultiTensorAdamW"), otype
         pw = ocfg.pop("paramwise_cfg", None) or {}
         keys = tuple(k for k, v in pw.get("custom_keys", {}).items() if v.get("decay_mult", 1.0) == 0.0)
         self.model = model
@@ -439,7 +440,18 @@ class Trainer:
             for b in model.buffers():
                 if b.numel():
                     dist.broadcast(b, src=0)
-        self.opt = FlatAdamW(self.flat, **ocfg)
+        if otype == "AdamW":
+            self.opt = FlatAdamW(self.flat, **ocfg)
+        else:
+            # optim.MultiTensorAdamW on the same parameters (the flat buffers stay the exchange's): its options -- moments in
+            # 8 bits -- come with the Python schedule; the C step engine runs FlatAdamW's kernel
+            from .optim import MultiTensorAdamW
+            decays = self.flat.decay_ranges()
+            decayed = [any(a <= o < b for a, b in decays) for o in self.flat.offsets]
+            wd = ocfg.pop("weight_decay", 0.05)
+            sets = [dict(params=[p for p, d in zip(self.flat.params, decayed) if d == want], weight_decay=wd if want else 0.0)
+                    for want in (True, False)]
+            self.opt = MultiTensorAdamW([g for g in sets if g["params"]], **ocfg)
         self.grad_clip = dict(GRAD_CLIP if grad_clip is None else grad_clip)
         self.lr_schedule = lr_schedule          # e.g. CyclicLr(base_lr, max_iters): lr set before every step
         self.iter = 0
@@ -447,7 +459,7 @@ class Trainer:
         self.explicit_schedule = self.flat.flat.is_cuda
         # the whole step as one C call (geomae_amd/engine.py, csrc/engine.hip); False = the Python explicit schedule
         # (same kernels, same order: kept as the A/B reference of the engine)
-        self.use_engine = self.flat.flat.is_cuda
+        self.use_engine = self.flat.flat.is_cuda and otype == "AdamW"
         self.engine = None
 
     def get_engine(self):
@@ -505,6 +517,21 @@ class Trainer:
         self.iter += 1
         return {k: losses[i] for i, k in enumerate(Det.LOSS_KEYS)}, gnorm
 
+    def _set_lr(self, lr):
+        if isinstance(self.opt, FlatAdamW):
+            self.opt.lr = lr
+        else:
+            for g in self.opt.param_groups:
+                g["lr"] = lr
+
+    def _clip_step(self, max_norm, grad_scale):
+        """Clip, update, zero the gradients; returns the gradient norm before clipping."""
+        if isinstance(self.opt, FlatAdamW):
+            return self.opt.fused_clip_step(max_norm, grad_scale, zero_grad=True)
+        self.opt.step(max_norm=max_norm or float("inf"), grad_scale=grad_scale)
+        self.flat.zero_grad()
+        return self.opt.grad_norm
+
     def train_step(self, points, next_points=None, **kw):
         """next_points: the batch of the FOLLOWING step (the same list object must be passed as `points`
         then); its voxelization / pillar sort is enqueued ahead of this step so that its count readback is
@@ -518,7 +545,7 @@ class Trainer:
             self.flat.zero_grad()
         self._grads_clean = False
         if self.lr_schedule is not None:
-            self.opt.lr = self.lr_schedule.lr_at(self.iter)
+            self._set_lr(self.lr_schedule.lr_at(self.iter))
         if getattr(self, "_prepack_flat_version", None) not in (None, self.flat.flat._version):
             self.model.backbone._packed.invalidate()        # someone wrote the flat parameter buffer since the pre-pack
         self._prepack_flat_version = None
@@ -572,7 +599,7 @@ class Trainer:
                 tap = getattr(self, "on_reduced_grad", None)
                 if tap is not None:                  # test tap: the summed gradient buffer the optimizer is about to read
                     tap(self.flat.grad)
-            gnorm = self.opt.fused_clip_step(self.grad_clip.get("max_norm", 0.0), 1.0 / world, zero_grad=True)
+            gnorm = self._clip_step(self.grad_clip.get("max_norm", 0.0), 1.0 / world)
             self._grads_clean = True
             packed = getattr(getattr(self.model, "backbone", None), "_packed", None)
             if explicit and packed is not None:

@@ -118,7 +118,8 @@ class DynamicScatterVFE(nn.Module):
         return (self.use_fused and seg is not None and self.training and features.is_cuda and not return_inv
                 and not self.return_point_feats and features.shape[1] == 5 and self._with_cluster_center
                 and self._with_voxel_center and not self._with_distance and self.rel_dist_scaler == 1.0
-                and [l.linear.out_features for l in self.vfe_layers] == [64, 128])
+                and [l.linear.out_features for l in self.vfe_layers] == [64, 128]
+                and all(isinstance(l.norm, nn.BatchNorm1d) for l in self.vfe_layers))
 
     # ---- explicit (autograd-free) schedule of the fused path: detector.train_step_explicit
     @torch.no_grad()

@@ -785,8 +785,8 @@ int geomae_adamw_step(float* params, float* grads, float* exp_avg, float* exp_av
  * geomae_multi_adamw_chunk() elements; first_chunk (host) [num_tensors + 1].  grads (host) [num_tensors]: device addresses,
  * NULL = the tensor has no gradient and is left as it is, its step too.  hyper_of (host) [num_tensors] indexes hypers (host)
  * [num_hypers]; lr_ptr (device, or NULL) replaces lr.  Gradients are scaled by grad_scale * (grad_scale_ptr ?
- * *grad_scale_ptr : 1) and, max_norm > 0, clipped to that norm over ALL tensors, whose pre-clip value grad_norm_out (device,
- * or NULL) receives.  skip_nonfinite != 0: a norm that is not finite leaves every parameter, moment and step as it was.
+ * *grad_scale_ptr : 1) and, max_norm > 0, clipped to that norm over ALL tensors (infinity: not at all), whose pre-clip value grad_norm_out
+ * (device, or NULL) receives.  skip_nonfinite != 0: a norm that is not finite leaves every parameter, moment and step as it was.
  * The arguments are read before the call returns; the launches can be captured (gradients and lr_ptr at the same addresses). */
 enum { GEOMAE_DTYPE_F32 = 0, GEOMAE_DTYPE_BF16 = 1, GEOMAE_DTYPE_F16 = 2 };
 typedef struct GeomaeAdamwTensor {
@@ -817,6 +817,21 @@ int geomae_multi_adamw_step(const GeomaeAdamwTensor* table, const int32_t* chunk
 int geomae_adamw_moments8(const uint8_t* exp_avg, const uint8_t* exp_avg_exponent, const uint8_t* exp_avg_sq,
                           const uint8_t* exp_avg_sq_exponent, int64_t num_elems, void* exp_avg_out, void* root_out,
                           geomaeStream_t stream);
+
+/* ------------------------------------------------------------------ group norm with an activation, channels last
+ * x, y, dy, dx: [n][rows][c] of `dtype` (GEOMAE_DTYPE_*); a group is c / groups neighbouring channels of a sample (at most
+ * 1024 groups).  y = act(gamma (x - mean) / sqrt(var + eps) + beta), var biased; gamma, beta [c] of weight_dtype, or NULL (1, 0).
+ * stats [n][groups][2] fp64 receives (mean, 1 / sqrt(var + eps)): the backward pass reads it.  dgamma, dbeta [c] of
+ * weight_dtype, or NULL.  ReLU's derivative at 0 is 0; gelu is the erf form.  workspace: the forward and the backward pass need
+ * geomae_group_norm_workspace_bytes(..., backward = 0 / 1) bytes each (-1: bad shape), 16-byte aligned. */
+enum { GEOMAE_ACT_NONE = 0, GEOMAE_ACT_RELU = 1, GEOMAE_ACT_SILU = 2, GEOMAE_ACT_GELU = 3 };
+int64_t geomae_group_norm_workspace_bytes(int32_t n, int64_t rows, int32_t c, int32_t groups, int32_t dtype, int32_t backward);
+int geomae_group_norm_forward(const void* x, int32_t dtype, int32_t n, int64_t rows, int32_t c, int32_t groups, const void* gamma,
+                              const void* beta, int32_t weight_dtype, double eps, int32_t activation, void* y, double* stats,
+                              void* workspace, int64_t workspace_bytes, geomaeStream_t stream);
+int geomae_group_norm_backward(const void* x, const void* dy, int32_t dtype, int32_t n, int64_t rows, int32_t c, int32_t groups,
+                               const void* gamma, const void* beta, int32_t weight_dtype, int32_t activation, const double* stats,
+                               void* dx, void* dgamma, void* dbeta, void* workspace, int64_t workspace_bytes, geomaeStream_t stream);
 
 /* BatchNorm parameter gradients from the LOCAL backward sums of the fused VFE (naiveSyncBN1d at world > 1: they are
  * added before the sums are all-reduced for the input gradient): d_beta[c] += bsums[c], d_gamma[c] += bsums[C + c]. */
