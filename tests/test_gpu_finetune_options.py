@@ -1,0 +1,137 @@
+"""The fine-tune model with group norms, trained by MultiTensorAdamW: the operators together, as a training run uses them."""
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."))
+from geomae_amd import synth  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+RANGE = (-50.0, -50.0, -5.0, 50.0, 50.0, 3.0)
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda:0")
+
+
+class FeatureLoss(torch.nn.Module):
+    """A linear head with a squared loss on the neck's features: what a Trainer needs of a detector, without its targets."""
+
+    def __init__(self, net, channels):
+        super().__init__()
+        self.net, self.head = net, torch.nn.Conv2d(channels, 4, 1)
+
+    def forward_train(self, points, img_metas=None):
+        return {"loss": (self.head(self.net.extract_feat(points)[0]) ** 2).mean()}
+
+
+def build(dev, seed=0):
+    import geomae_amd
+    from geomae_amd.configs import pre_sst_model
+    cfg = pre_sst_model(num_blocks=1, conv_out_channels=(32, 32, 64), layer_nums=(1, 1, 1))
+    cfg.pop("bbox_head")
+    gn = dict(type="GN", num_groups=8, eps=1e-3)
+    cfg["backbone"]["norm_cfg"], cfg["neck"]["norm_cfg"] = gn, gn
+    cfg["middle_encoder"]["shuffle_voxels"] = False
+    torch.manual_seed(seed)
+    return FeatureLoss(geomae_amd.build_model(cfg), 384).to(dev).train()
+
+
+def frames(dev, k):
+    return [torch.as_tensor(synth.lidar_frame(70 + 2 * k + i, beams=16, n_az=300, pc_range=RANGE), device=dev) for i in range(2)]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_trainer_steps_are_the_optimizers(dev, bits, tmp_path):
+    """Three Trainer steps of the group-norm model: finite losses and norms, every parameter with a gradient moves; each step is
+    exactly MultiTensorAdamW's on the same gradients; a checkpoint continues with the same parameters."""
+    from geomae_amd.optim import MultiTensorAdamW
+    from geomae_amd.train import Trainer
+    ocfg = dict(type="MultiTensorAdamW", lr=1e-4, betas=(0.9, 0.999), weight_decay=0.05, state_bits=bits, seed=3,
+                paramwise_cfg=dict(custom_keys={"norm": dict(decay_mult=0.0)}))
+    model = build(dev)
+    tr = Trainer(model, ocfg, grad_clip=dict(max_norm=1.0, norm_type=2), lr_schedule=None)
+    assert isinstance(tr.opt, MultiTensorAdamW) and tr.opt.state_bits == bits and not tr.use_engine
+    params = [p for g in tr.opt.param_groups for p in g["params"]]
+    assert {id(p) for p in params} == {id(p) for p in model.parameters()}
+    names = {id(p): n for n, p in model.named_parameters()}
+    undecayed = [names[id(p)] for g in tr.opt.param_groups if g["weight_decay"] == 0.0 for p in g["params"]]
+    assert undecayed and all("norm" in n for n in undecayed)
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    sizes = [len(g["params"]) for g in tr.opt.param_groups]
+    other = MultiTensorAdamW([dict(params=twins[:sizes[0]], weight_decay=0.05), dict(params=twins[sizes[0]:], weight_decay=0.0)], lr=1e-4,
+                             state_bits=bits, seed=3)
+    start = [p.detach().clone() for p in params]
+    grads, clip = [], tr._clip_step
+
+    def tap(*args):
+        grads.append([p.grad.clone() for p in params])
+        return clip(*args)
+    tr._clip_step = tap
+    for k in range(3):
+        losses, gnorm = tr.train_step(frames(dev, k))
+        norm = float(gnorm)
+        assert np.isfinite(float(losses["loss"])) and np.isfinite(norm) and norm > 0
+        want = np.sqrt(sum(float((g.double() ** 2).sum()) for g in grads[-1]))
+        assert abs(norm - want) <= 2.0 ** -23 * want
+        for q, g in zip(twins, grads[-1]):
+            q.grad = g
+        other.step(max_norm=1.0)
+        assert all(torch.equal(p, q) for p, q in zip(params, twins)), k
+        assert not tr.flat.grad.any()
+    moved = [not torch.equal(p, s) for p, s in zip(params, start)]
+    has = [any(bool(g[i].any()) for g in grads) for i in range(len(params))]
+    assert all(m for m, h in zip(moved, has) if h) and sum(has) > 0.9 * len(has)
+    tr.save_checkpoint(str(tmp_path / "run.pth"))
+    again = Trainer(build(dev, seed=1), ocfg, grad_clip=dict(max_norm=1.0, norm_type=2))
+    again.load_checkpoint(str(tmp_path / "run.pth"))
+    assert all(torch.equal(a, b) for a, b in zip(model.state_dict().values(), again.model.state_dict().values()))
+    mine = [p for g in again.opt.param_groups for p in g["params"]]
+    for p, q, g in zip(params, mine, grads[0]):
+        p.grad.copy_(g)
+        q.grad.copy_(g)
+    clip(1.0, 1.0)
+    again._clip_step(1.0, 1.0)
+    assert all(torch.equal(p, q) for p, q in zip(params, mine))
+
+
+def test_group_norm_model_has_the_gradients_of_its_definition(dev):
+    """The neck's output and all gradients of the conv stages, against the same convolutions with the group norm written out in
+    torch: the two differ by fp32 roundings, which the convolutions' own sums (of up to 576 products) amplify."""
+    from geomae_amd.norm import GroupNormAct
+    model = build(dev)
+    canvas = torch.randn(2, 128, 104, 104, device=dev)                  # (the neck joins strides of 2, 4, 8: a multiple of 8)
+
+    def run():
+        model.zero_grad(set_to_none=True)
+        x, outs = canvas, []
+        for blk in model.net.backbone.conv_blocks:
+            x = blk(x)
+            outs.append(x)
+        y = model.net.neck(tuple(outs))[0]
+        (y * torch.linspace(-1, 1, y.shape[1], device=dev)[:, None, None]).sum().backward()
+        return y.detach(), {n: p.grad.clone() for n, p in model.named_parameters() if p.grad is not None}
+
+    def plain(self, x):
+        n, c = x.shape[:2]
+        v = x.double().contiguous().reshape(n, self.num_groups, -1)
+        v = (v - v.mean(2, keepdim=True)) / torch.sqrt(v.var(2, keepdim=True, unbiased=False) + self.eps)
+        return (v.reshape(x.shape) * self.weight[:, None, None] + self.bias[:, None, None]).clamp(min=0).float()
+    got, g1 = run()
+    kernel = GroupNormAct.forward
+    GroupNormAct.forward = plain
+    try:
+        want, g2 = run()
+    finally:
+        GroupNormAct.forward = kernel
+    # eight layers of convolution and norm: sqrt(576) roundings each, at most a factor two per layer and direction
+    bound = 16 * 24 * 2.0 ** -24 * 4
+    assert float((got - want).norm() / want.norm()) <= bound
+    assert g1.keys() == g2.keys() and len(g1) > 20
+    for k in g1:
+        # ReLU masks next to zero may differ between two fp32 convolutions: a share of 1e-6 of the elements, in the 2-norm 1e-3
+        assert float((g1[k] - g2[k]).norm()) <= (bound + 1e-3) * float(g2[k].norm()), k
