@@ -350,6 +350,26 @@ def load(path=None):
     return lib
 
 
+_host = None
+
+
+def host():
+    """The Python extension _host.so (csrc/host.cpp), bound to the loaded library's entry points."""
+    global _host
+    if _host is None:
+        lib = load()
+        import torch  # noqa: F401  (its libraries first: the extension links to them)
+        try:
+            from . import _host as ext
+        except ImportError as e:
+            raise GeomaeLibraryError(f"geomae_amd/_host.so cannot be loaded ({e}): build it with `python -m geomae_amd.csrc.build`") from e
+        names = ("geomae_multi_adamw_step", "geomae_group_norm_workspace_bytes", "geomae_group_norm_forward",
+                 "geomae_group_norm_backward", "geomae_last_error")
+        ext.bind({n: ctypes.cast(getattr(lib, n), c_void_p).value for n in names}, GeomaeLibraryError)
+        _host = ext
+    return _host
+
+
 def check(rc, what):
     if rc != 0:
         msg = load().geomae_last_error().decode("utf-8", "replace")

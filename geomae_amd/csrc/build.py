@@ -1,4 +1,4 @@
-"""Build libgeomae_hip.so in-tree with hipcc for gfx950 (cross-compiles without a GPU)."""
+"""Build libgeomae_hip.so (hipcc for gfx950, cross-compiles without a GPU) and the Python extension _host.so (g++) in-tree."""
 import glob
 import os
 import subprocess
@@ -28,6 +28,22 @@ def flags_for(src):
     return FLAGS + ([] if os.path.basename(src) in KEEPS_PACKED else NO_PACKED) + ["-ffp-contract=" + ("fast" if os.path.basename(src) in CONTRACT_FAST else "off")]
 
 
+HOST_SRC, HOST_OUT = os.path.join(HERE, "host.cpp"), os.path.join(PKG, "_host.so")
+
+
+def host_command():
+    """host.cpp against torch's headers and libraries; it reaches libgeomae_hip through addresses that _lib.host() binds."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    rocm = os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")
+    inc = [f for d in cpp_extension.include_paths() + [rocm, sysconfig.get_paths()["include"]] for f in ("-isystem", d)]
+    return (["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-DTORCH_EXTENSION_NAME=_host", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + inc +
+            [HOST_SRC, "-o", HOST_OUT, "-L" + lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"])
+
+
 def sources():
     return sorted(glob.glob(os.path.join(HERE, "*.hip")))
 
@@ -45,6 +61,8 @@ def build(force=False, verbose=False):
     os.makedirs(objdir, exist_ok=True)
     jobs = []
     objs = []
+    if force or _newer(HOST_OUT, [HOST_SRC, os.path.abspath(__file__), os.path.join(ROOT, "include", "geomae_hip.h")]):
+        jobs.append(host_command())                # (first: the longest of them)
     for src in sources():
         obj = os.path.join(objdir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)

@@ -1093,25 +1093,9 @@ def recover_bev(feat, coors, batch_size, ny, nx):
 
 
 # ------------------------------------------------------------------------------------ group norm + activation
-_GN_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_GN_ACT = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
-
-
-def _gn_rows(x):
-    """(samples, rows per sample, channels) of a dense channels-last [N, C, *] tensor."""
-    n, c = x.shape[0], x.shape[1]
-    return n, (x.numel() // (n * c) if x.numel() else 0), c
-
-
 def _channels_last(t):
+    """t.movedim(1, -1) is contiguous."""
     return t.dim() == 2 and t.is_contiguous() or t.dim() > 2 and t.movedim(1, -1).is_contiguous()
-
-
-def _channels_last_empty(x):
-    """A tensor of x's shape in channels-last memory."""
-    if x.dim() == 2:
-        return torch.empty_like(x, memory_format=torch.contiguous_format)
-    return torch.empty((x.shape[0], *x.shape[2:], x.shape[1]), dtype=x.dtype, device=x.device).movedim(-1, 1)
 
 
 def _to_channels_last(x):
@@ -1119,86 +1103,11 @@ def _to_channels_last(x):
     return x.movedim(1, -1).contiguous().movedim(-1, 1)
 
 
-def _gn_forward(x, num_groups, weight, bias, eps, act):
-    lib, (n, rows, c) = _lib.load(), _gn_rows(x)
-    dt, wdt = _GN_DTYPE[x.dtype], _GN_DTYPE[weight.dtype if weight is not None else torch.float32]
-    y = _channels_last_empty(x)
-    if x.numel() == 0:
-        return y, None
-    wsb = lib.geomae_group_norm_workspace_bytes(n, rows, c, num_groups, dt, 0)
-    if wsb < 0:
-        check(wsb, "geomae_group_norm_workspace_bytes")
-    stats = torch.empty(2 * n * num_groups, dtype=torch.float64, device=x.device)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        check(lib.geomae_group_norm_forward(_ptr(x), dt, n, rows, c, num_groups, _ptr(weight), _ptr(bias), wdt, eps, act, _ptr(y),
-                                            _ptr(stats), _ptr(ws), wsb, _stream()),
-              "geomae_group_norm_forward")
-    return y, stats
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, num_groups, eps, act):
-        y, stats = _gn_forward(x, num_groups, weight, bias, eps, act)
-        ctx.save_for_backward(x, weight, bias, stats)
-        ctx.num_groups, ctx.act = num_groups, act
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
-        db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
-        dx = _channels_last_empty(x)
-        if x.numel() == 0:
-            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None, None
-        if not _channels_last(dy):
-            dy = _channels_last_empty(dy).copy_(dy)
-        lib, (n, rows, c) = _lib.load(), _gn_rows(x)
-        dt, wdt = _GN_DTYPE[x.dtype], _GN_DTYPE[weight.dtype if weight is not None else torch.float32]
-        wsb = lib.geomae_group_norm_workspace_bytes(n, rows, c, ctx.num_groups, dt, 1)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
-        with torch.cuda.device(x.device):
-            check(lib.geomae_group_norm_backward(_ptr(x), _ptr(dy), dt, n, rows, c, ctx.num_groups, _ptr(weight), _ptr(bias), wdt, ctx.act,
-                                                 _ptr(stats), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), wsb, _stream()),
-                  "geomae_group_norm_backward")
-        return dx, dw, db, None, None, None
-
-
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None):
     """act(group_norm(x)) of a channels-last [N, C, *] tensor (x.movedim(1, -1) contiguous: images in
-    torch.channels_last, [N, C] rows), differentiable.  x float32 / bfloat16 / float16; weight, bias [C] of one dtype, or None;
-    activation None, "relu", "silu" or "gelu" (erf).  y has x's dtype and layout; statistics and sums are fp64 / fp32."""
-    if not x.is_cuda:
-        raise RuntimeError("x must be a CUDA tensor (geomae_amd has no CPU path)")
-    if x.dim() < 2:
-        raise RuntimeError(f"x must be [N, C, *], got {tuple(x.shape)}")
-    if x.dtype not in _GN_DTYPE:
-        raise RuntimeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    if not _channels_last(x):
-        raise RuntimeError("x must be in channels-last memory (x.movedim(1, -1) contiguous)")
-    if activation not in _GN_ACT:
-        raise RuntimeError(f"activation must be None, 'relu', 'silu' or 'gelu', got {activation!r}")
-    c = x.shape[1]
-    if num_groups < 1 or c % num_groups:
-        raise RuntimeError(f"{c} channels do not divide into {num_groups} groups")
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None:
-            _check_input(t, name)
-            if t.shape != (c,) or t.dtype not in _GN_DTYPE or t.device != x.device:
-                raise RuntimeError(f"{name} must be [{c}] float32, bfloat16 or float16 on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise RuntimeError(f"weight and bias must have one dtype, got {weight.dtype} and {bias.dtype}")
-    if weight is None and bias is not None:
-        raise RuntimeError("a bias needs a weight")
-    if eps < 0:
-        raise RuntimeError(f"eps must not be negative, got {eps}")
-    act = _GN_ACT[activation]
-    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad):
-        return _GroupNormAct.apply(x, weight, bias, int(num_groups), float(eps), act)
-    return _gn_forward(x, int(num_groups), weight, bias, float(eps), act)[0]
+    torch.channels_last, [N, C] rows), differentiable once.  x float32 / bfloat16 / float16; weight, bias [C] of one dtype, or
+    None; activation None, "relu", "silu" or "gelu" (erf).  y has x's dtype and layout; statistics and sums are fp64 / fp32."""
+    return _lib.host().group_norm_act(x, num_groups, weight, bias, eps, activation)
 
 
 # ------------------------------------------------------------------------------------ fused SST layer

@@ -51,7 +51,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         self.state_bits, self.master_weights, self.seed = int(state_bits), bool(master_weights), int(seed)
         if not 0 <= self.seed < 2 ** 32:
             raise ValueError("seed must be in [0, 2**32)")
-        self._arena, self._table, self._building = None, None, True
+        self._arena, self._table, self._building, self._captured, self._retired = None, None, True, False, []
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         self._building = False
@@ -100,6 +100,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     def _build(self):
         """Moments of all parameters in one arena per kind, each parameter's part starting at a multiple of 32 elements; a
         parameter's state tensors are views of it in the parameter's own layout.  Parameters that were there keep theirs."""
+        self._retire()
         params, old = self._params(), self._arena
         dev = params[0].device
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
@@ -137,12 +138,16 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         within = torch.arange(first[-1], dtype=torch.int64) - torch.tensor(first[:-1], dtype=torch.int64)[tensor.long()]
         self._chunks = torch.stack([tensor, within.int()], 1).contiguous().to(dev)
         n = len(params)
-        self._first_chunk = (ctypes.c_int64 * (n + 1))(*first)
-        self._grad_ptrs, self._hyper_of = (ctypes.c_void_p * n)(), (ctypes.c_int32 * n)()
+        self._first_chunk = first
         ws = lib.geomae_multi_adamw_workspace_bytes(n)
         self._workspace = torch.empty(ws, dtype=torch.uint8, device=dev)
         self._norm_word = torch.zeros((), dtype=torch.float32, device=dev)
         self._fill_table()
+
+    def _retire(self):
+        """What a captured step may still read and write is kept as long as this optimizer."""
+        if self._captured:
+            self._retired.append((self._table, self._arena, self._chunks, self._workspace, self._norm_word))
 
     @staticmethod
     def _part(flat, off, p):
@@ -161,8 +166,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         return out
 
     def _fill_table(self):
-        """The device table of addresses.  A table that a captured step may still read is kept as long as this optimizer."""
-        params, a, rows = self._params(), self._arena, None
+        """The device table of addresses."""
+        params, a = self._params(), self._arena
         rows = (_lib.GeomaeAdamwTensor * len(params))()
         for i, (p, off) in enumerate(zip(params, self.offsets)):
             r = rows[i]
@@ -176,10 +181,11 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             r.step = a["step"].data_ptr() + 8 * i
             r.numel, r.dtype, r.index = p.numel(), _DTYPE[p.dtype], i
         host = torch.frombuffer(bytearray(rows), dtype=torch.uint8)
-        self._retired = getattr(self, "_retired", []) + ([self._table] if self._table is not None else [])
+        self._retire()
         self._table = host.to(params[0].device)
-        self._where = [p.data_ptr() for p in params]
-        self._layout = [(p.shape, p.stride(), p.dtype) for p in params]
+        self._layout = [(p.shape, p.stride(), p.dtype, p.device) for p in params]
+        self._plan = _lib.host().AdamwPlan([p.data_ptr() for p in params], self._first_chunk, self._table.data_ptr(), self._chunks.data_ptr(),
+                                           self._workspace.data_ptr(), self._workspace.numel(), self._norm_word.data_ptr(), self.state_bits)
 
     # ------------------------------------------------------------------------------------------------ the step
     @torch.no_grad()
@@ -193,71 +199,26 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        params = self._params()
-        dev = params[0].device
-        where = [p.data_ptr() for p in params]
-        if where != self._where:
-            if [(p.shape, p.stride(), p.dtype) for p in params] != self._layout:
-                raise RuntimeError("MultiTensorAdamW: a parameter changed its shape, layout or dtype; make a new optimizer")
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("MultiTensorAdamW: a parameter's storage moved; take one step outside the capture first")
-            self._check_params(params)
-            self._fill_table()
-        keep, i = [], 0
-        hypers, number = [], {}
-        for group in self.param_groups:
-            lr = group["lr"]
-            key = (lr.data_ptr() if torch.is_tensor(lr) else float(lr), torch.is_tensor(lr), *map(float, group["betas"]),
-                   float(group["eps"]), float(group["weight_decay"]))
-            k = number.get(key)
-            if k is None:
-                self._check_hyper(group)
-                k = number[key] = len(hypers)
-                hypers.append(key)
-            for p in group["params"]:
-                g = p.grad
-                if g is None:
-                    self._grad_ptrs[i] = None
-                else:
-                    if g.stride() != p.stride() or g.dtype != p.dtype or g.layout != torch.strided or g.device != dev:
-                        g = self._like(g, p)
-                        keep.append(g)
-                    self._grad_ptrs[i] = g.data_ptr()
-                    self._hyper_of[i] = k
-                i += 1
-        hyper_rows = (_lib.GeomaeAdamwHyper * max(1, len(hypers)))()
-        for row, (lr, is_tensor, b1, b2, eps, wd) in zip(hyper_rows, hypers):
-            row.lr, row.lr_ptr = (0.0, lr) if is_tensor else (lr, None)
-            row.beta1, row.beta2, row.eps, row.weight_decay = b1, b2, eps, wd
-        scale_ptr, scale = None, 1.0
-        if torch.is_tensor(grad_scale):
-            if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev:
-                raise RuntimeError("MultiTensorAdamW: a tensor grad_scale must be one float32 value on the parameters' GPU")
-            scale_ptr = grad_scale.data_ptr()
-        else:
-            scale = float(grad_scale)
-        wants_norm = float(max_norm or 0.0) > 0.0 or skip_nonfinite
-        with torch.cuda.device(dev):
-            stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-            _lib.check(_lib.load().geomae_multi_adamw_step(
-                _ptr(self._table), _ptr(self._chunks), self._first_chunk, len(params), self._grad_ptrs, self._hyper_of,
-                ctypes.addressof(hyper_rows), len(hypers), self.state_bits, float(max_norm or 0.0), scale, scale_ptr,
-                int(bool(skip_nonfinite)), self.seed, _ptr(self._norm_word) if wants_norm else None, _ptr(self._workspace),
-                self._workspace.numel(), stream), "geomae_multi_adamw_step")
-        torch.autograd.graph.increment_version(params)
-        if wants_norm:
+        scale, scale_tensor = (1.0, grad_scale) if torch.is_tensor(grad_scale) else (float(grad_scale), None)
+        max_norm = float(max_norm or 0.0)
+        self._plan.seed = self.seed
+        self._captured = self._captured or torch.cuda.is_current_stream_capturing()
+        if not self._plan.step(self.param_groups, max_norm, scale, scale_tensor, skip_nonfinite):
+            self._find_params()
+            self._plan.step(self.param_groups, max_norm, scale, scale_tensor, skip_nonfinite)
+        if max_norm > 0.0 or skip_nonfinite:
             self.grad_norm = self._norm_word
         return loss
 
-    @staticmethod
-    def _like(g, p):
-        """A gradient in another layout than its parameter's, as a copy in the parameter's."""
-        if g.layout != torch.strided:
-            raise RuntimeError("MultiTensorAdamW: sparse gradients are not supported")
-        if g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
-            raise RuntimeError(f"MultiTensorAdamW: a gradient ({g.dtype}, {tuple(g.shape)}, {g.device}) does not match its parameter "
-                               f"({p.dtype}, {tuple(p.shape)}, {p.device})")
-        return torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
+    def _find_params(self):
+        """A parameter is not where the device table says: make the table anew."""
+        params = self._params()
+        if [(p.shape, p.stride(), p.dtype, p.device) for p in params] != self._layout:
+            raise RuntimeError("MultiTensorAdamW: a parameter changed its shape, layout, dtype or device; make a new optimizer")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("MultiTensorAdamW: a parameter's storage moved; take one step outside the capture first")
+        self._check_params(params)
+        self._fill_table()
 
     # ------------------------------------------------------------------------------------------------ state
     def moments(self):
