@@ -28,12 +28,11 @@ namespace geomae {
 
 constexpr int kMaThreads = 256, kMaVec = 4, kMaIters = 4;
 constexpr int kMaChunk = kMaThreads * kMaVec * kMaIters;             // elements of a workgroup
-constexpr int kMaTensors = 256;                                      // gradient addresses of a launch (2 KB of arguments)
-constexpr int kMaHypers = 16;                                        // distinct hyper-parameter sets of a launch
-constexpr int kMaNormGrid = 1024;                                    // workgroups (= partial sums) of a norm launch
+constexpr int kMaTensors = 384;                                      // gradient addresses of a launch (3 of its 4 KB of arguments)
+constexpr int kMaHypers = 8;                                         // distinct hyper-parameter sets of a launch
+constexpr int kMaNormGrid = 1024;                                    // workgroups (= partial sums) of a norm, over all launches
 
-struct MaScalars { float decay, w1, b2, omb2, bc2_sqrt, eps, step_size; uint32_t key; };
-struct MaControl { float coef; int32_t skip; };
+struct MaScalars { float decay, w1, b2, omb2, bc2_sqrt, inv_bc2_sqrt, eps, step_size; uint32_t key; };
 
 __host__ __device__ __forceinline__ uint32_t ma_mix(uint32_t x) {
     x = (x ^ (x >> 15)) * 0xBB67AE85u;
@@ -54,207 +53,235 @@ template <> __device__ __forceinline__ uint16_t ma_narrow<uint16_t>(float x) {  
     return x != x ? (uint16_t)((b >> 16) | 0x40) : (uint16_t)((b + 0x7fff + ((b >> 16) & 1)) >> 16);
 }
 
-template <typename T>
-__device__ __forceinline__ void ma_load(const T* p, int64_t e, int64_t n, float (&out)[kMaVec]) {
-    if (e + kMaVec <= n) {
-        const MaPack<T, kMaVec> w = *reinterpret_cast<const MaPack<T, kMaVec>*>(p + e);
+// kMaVec elements at offset o of a chunk that has `left` of them; FULL: all of the workgroup's
+template <bool FULL, typename T>
+__device__ __forceinline__ void ma_load(const T* p, int o, int left, float (&out)[kMaVec]) {
+    if (FULL || o + kMaVec <= left) {
+        const MaPack<T, kMaVec> w = *reinterpret_cast<const MaPack<T, kMaVec>*>(p + o);
 #pragma unroll
         for (int i = 0; i < kMaVec; ++i) out[i] = ma_float<T>(w.v[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < kMaVec; ++i) out[i] = e + i < n ? ma_float<T>(p[e + i]) : 0.f;
+        for (int i = 0; i < kMaVec; ++i) out[i] = o + i < left ? ma_float<T>(p[o + i]) : 0.f;
     }
 }
-template <typename T>
-__device__ __forceinline__ void ma_store(T* p, int64_t e, int64_t n, const float (&x)[kMaVec]) {
-    if (e + kMaVec <= n) {
+template <bool FULL, typename T>
+__device__ __forceinline__ void ma_store(T* p, int o, int left, const float (&x)[kMaVec]) {
+    if (FULL || o + kMaVec <= left) {
         MaPack<T, kMaVec> w;
 #pragma unroll
         for (int i = 0; i < kMaVec; ++i) w.v[i] = ma_narrow<T>(x[i]);
-        *reinterpret_cast<MaPack<T, kMaVec>*>(p + e) = w;
+        *reinterpret_cast<MaPack<T, kMaVec>*>(p + o) = w;
     } else {
 #pragma unroll
         for (int i = 0; i < kMaVec; ++i)
-            if (e + i < n) p[e + i] = ma_narrow<T>(x[i]);
+            if (o + i < left) p[o + i] = ma_narrow<T>(x[i]);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ 8-bit moments
-// largest finite magnitude of the 8 lanes x 4 elements of a block
-__device__ __forceinline__ float ma_block_max(const float (&x)[kMaVec]) {
-    float a = 0.f;
+// A magnitude in units of its block's scale, times 2^-120, has the codes' exponent field and digits at the top of its fp32 bits,
+// the even spacing below 2^-6 as fp32's own subnormal numbers.  Decoding is a shift and an exponent, encoding a shift too: the
+// draw, (2 u + 1) in units of 2^-17 of a step, is added below the code's last digit and carries into it.  (The largest code and
+// above, infinity and NaN end at or over the NaN code and are clamped to it.)
+__device__ __forceinline__ uint32_t ma_magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// largest finite magnitude (its bits) of the 8 lanes x 4 elements of a block
+__device__ __forceinline__ uint32_t ma_block_max(const float (&x)[kMaVec]) {
+    uint32_t a = 0;
 #pragma unroll
-    for (int i = 0; i < kMaVec; ++i) {
-        const float y = fabsf(x[i]);
-        a = fmaxf(a, y < INFINITY ? y : 0.f);
+    for (int i = 0; i < kMaVec; ++i) a = max(a, ma_magnitude(x[i]));
+    if (__builtin_expect(a >= 0x7f800000u, 0)) {
+        a = 0;
+#pragma unroll
+        for (int i = 0; i < kMaVec; ++i) a = max(a, ma_magnitude(x[i]) < 0x7f800000u ? ma_magnitude(x[i]) : 0u);
     }
-    a = fmaxf(a, dpp_mov<kDppXor1>(a));
-    a = fmaxf(a, dpp_mov<kDppXor2>(a));
-    return fmaxf(a, dpp_mov<kDppHalfMirror>(a));
+    a = max(a, (uint32_t)dpp_mov<kDppXor1>((int)a));
+    a = max(a, (uint32_t)dpp_mov<kDppXor2>((int)a));
+    return max(a, (uint32_t)dpp_mov<kDppHalfMirror>((int)a));
 }
 template <bool SIGNED>
-__device__ __forceinline__ int ma_exponent(float largest) {          // + 0x1fffff / 0x0fffff: carries above 1.75 / 1.875
-    const int e = (int)((__float_as_uint(largest) + (SIGNED ? 0x1fffffu : 0x0fffffu)) >> 23);
+__device__ __forceinline__ int ma_exponent(uint32_t largest) {       // + 0x1fffff / 0x0fffff: carries above 1.75 / 1.875
+    const int e = (int)((largest + (SIGNED ? 0x1fffffu : 0x0fffffu)) >> 23);
     return e < 16 ? 16 : (e > 254 ? 254 : e);
 }
-__device__ __forceinline__ float ma_unscale(int e) { return __uint_as_float((uint32_t)(e - 8) << 23); }     // 2^(E - 135)
 __device__ __forceinline__ float ma_scale(int e) { return __uint_as_float((uint32_t)(262 - e) << 23); }     // 2^(135 - E)
 
-// y >= 0 in units of the block's scale -> the code value it is held as
-template <int DIGITS>
-__device__ __forceinline__ float ma_round(float y, uint32_t u16) {
-    int place = (int)(__float_as_uint(y) >> 23);
-    place = place < 121 ? 121 : place;                               // below 2^-6 the codes are evenly spaced
-    const float inv_step = __uint_as_float((uint32_t)(254 + DIGITS - place) << 23);
-    const float step = __uint_as_float((uint32_t)(place - DIGITS) << 23);
-    return floorf(__fadd_rn(y * inv_step, ((float)u16 + 0.5f) * 0x1p-16f)) * step;
-}
 __device__ __forceinline__ uint32_t ma_code_signed(const float (&x)[kMaVec], float scale, const uint32_t (&draw)[kMaVec]) {
-    float q[kMaVec];
-    uint32_t bad = 0;
+    uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < kMaVec; ++i) {
-        const float y = fabsf(x[i]) * scale;
-        q[i] = copysignf(ma_round<3>(y, draw[i] & 0xffffu), x[i]);
-        if (!(fabsf(x[i]) < INFINITY)) bad |= 0x7fu << (8 * i), q[i] = 0.f;
+        const uint32_t z = __float_as_uint(fabsf(x[i]) * scale * 0x1p-120f);
+        const uint32_t c = min((z + (((draw[i] & 0xffffu) << 4) | 8u)) >> 20, 0x7fu);
+        w |= (c | ((__float_as_uint(x[i]) >> 24) & 0x80u)) << (8 * i);
     }
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);   // exact: q is a code's value already
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
-    return (uint32_t)w | bad;
+    return w;
 }
 __device__ __forceinline__ uint32_t ma_code_root(const float (&x)[kMaVec], float scale, const uint32_t (&draw)[kMaVec]) {
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < kMaVec; ++i) {
-        const float y = x[i] * scale;
-        float q = ma_round<4>(y, draw[i] >> 16);
-        if (q == 0.f && x[i] > 0.f) q = 0x1p-10f;
-        uint32_t c = q >= 0x1p-6f ? (__float_as_uint(q) >> 19) - 1920u : (uint32_t)(q * 0x1p10f);
-        if (!(x[i] < INFINITY)) c = 255u;
+        const uint32_t z = __float_as_uint(x[i] * scale * 0x1p-120f);
+        const uint32_t c = min(max((z + ((draw[i] >> 13 & ~7u) | 4u)) >> 19, min(__float_as_uint(x[i]), 1u)), 255u);
         w |= c << (8 * i);
     }
     return w;
 }
-__device__ __forceinline__ void ma_value_signed(uint32_t w, float unscale, float (&out)[kMaVec]) {
+__device__ __forceinline__ void ma_value_signed(uint32_t w, int e, float (&out)[kMaVec]) {
+    const float unscale = __uint_as_float((uint32_t)(e - 8) << 23);  // 2^(E - 135)
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
     out[0] = a[0] * unscale; out[1] = a[1] * unscale; out[2] = b[0] * unscale; out[3] = b[1] * unscale;
 }
-__device__ __forceinline__ void ma_value_root(uint32_t w, float unscale, float (&out)[kMaVec]) {
+__device__ __forceinline__ void ma_value_root(uint32_t w, int e, float (&out)[kMaVec]) {
 #pragma unroll
-    for (int i = 0; i < kMaVec; ++i) {
-        const uint32_t c = (w >> (8 * i)) & 255u;
-        const float f = c == 255u ? NAN : __uint_as_float(c << 19) * 0x1p120f;     // 4 + 4 bits as an fp32 with that exponent bias
-        out[i] = f * unscale;
+    for (int i = 0; i < kMaVec; ++i) out[i] = ldexpf(__uint_as_float(((w >> (8 * i)) & 255u) << 19), e - 15);
+    if (__builtin_expect((((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u) != 0, 0)) {
+#pragma unroll
+        for (int i = 0; i < kMaVec; ++i)
+            if (((w >> (8 * i)) & 255u) == 255u) out[i] = NAN;
     }
 }
 
-// ------------------------------------------------------------------------------------------------ norm
-struct MaNormArgs {
-    const GeomaeAdamwTensor* rows;
-    const int32_t* chunks;              // [num chunks][2] = (tensor, chunk of that tensor)
-    double* partial;                    // one per workgroup
-    int32_t first_tensor, first_chunk, num_chunks;
-    const void* grads[kMaTensors];
-};
-
-template <typename T>
-__device__ __forceinline__ double ma_sumsq(const T* g, int64_t start, int64_t n) {
+// ------------------------------------------------------------------------------------------------ norm, per-tensor scalars
+template <bool FULL, typename T>
+__device__ __forceinline__ double ma_sumsq(const T* g, int left) {
     double acc = 0.0;
     float x[kMaIters][kMaVec];
 #pragma unroll
-    for (int it = 0; it < kMaIters; ++it) {
-        const int64_t e = start + (it * kMaThreads + threadIdx.x) * kMaVec;
-        ma_load<T>(g, e < n ? e : n, n, x[it]);
-    }
+    for (int it = 0; it < kMaIters; ++it) ma_load<FULL, T>(g, (it * kMaThreads + (int)threadIdx.x) * kMaVec, left, x[it]);
 #pragma unroll
     for (int it = 0; it < kMaIters; ++it)
 #pragma unroll
-        for (int i = 0; i < kMaVec; ++i) acc += (double)x[it][i] * (double)x[it][i];
+        for (int i = 0; i < kMaVec; ++i) acc = fma((double)x[it][i], (double)x[it][i], acc);
     return acc;
 }
+template <typename T>
+__device__ __forceinline__ double ma_sumsq(const void* g, int64_t start, int64_t n) {
+    const T* p = static_cast<const T*>(g) + start;
+    return n - start >= kMaChunk ? ma_sumsq<true, T>(p, kMaChunk) : ma_sumsq<false, T>(p, (int)(n - start));
+}
 
-__global__ __launch_bounds__(kMaThreads) void multi_sumsq_kernel(MaNormArgs a) {
+// the sum of squares of all gradients from its partial sums, in a fixed order, in every thread
+constexpr int kMaHeld = 4;              // partial sums that a thread loads ahead
+__device__ __forceinline__ void ma_load_partials(const double* partial, int count, double (&held)[kMaHeld]) {
+#pragma unroll
+    for (int k = 0; k < kMaHeld; ++k) {
+        const int i = k * kMaThreads + (int)threadIdx.x;
+        held[k] = i < count ? partial[i] : 0.0;
+    }
+}
+__device__ __forceinline__ double ma_sum_partials(const double* partial, int count, const double (&held)[kMaHeld]) {
     __shared__ double red[kMaThreads / kWave];
     double acc = 0.0;
-    for (int c = blockIdx.x; c < a.num_chunks; c += gridDim.x) {
-        const int32_t* at = a.chunks + 2 * ((int64_t)a.first_chunk + c);
-        const int t = at[0];
-        const int64_t start = (int64_t)at[1] * kMaChunk;
-        const void* g = a.grads[t - a.first_tensor];
-        if (!g) continue;
-        const int64_t n = a.rows[t].numel;
-        const int dtype = a.rows[t].dtype;
-        if (dtype == GEOMAE_DTYPE_F32) acc += ma_sumsq(static_cast<const float*>(g), start, n);
-        else if (dtype == GEOMAE_DTYPE_BF16) acc += ma_sumsq(static_cast<const uint16_t*>(g), start, n);
-        else acc += ma_sumsq(static_cast<const _Float16*>(g), start, n);
-    }
+#pragma unroll
+    for (int k = 0; k < kMaHeld; ++k) acc += held[k];
+    for (int i = kMaHeld * kMaThreads + (int)threadIdx.x; i < count; i += kMaThreads) acc += partial[i];
     acc = wave_sum(acc);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
     __syncthreads();
-    if (threadIdx.x == 0) a.partial[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+    return red[0] + red[1] + red[2] + red[3];
 }
 
-// ------------------------------------------------------------------------------------------------ per-tensor scalars
+// the factor of the gradients: scale and clipping
+struct MaFactor {
+    const double* partial;              // of the norm
+    int32_t num_partial, skip_nonfinite;
+    double grad_scale;
+    const float* grad_scale_ptr;
+    float max_norm;
+    float* grad_norm;                   // of the first launch: receives the norm
+};
+// false: the step is skipped
+__device__ __forceinline__ bool ma_factor(const MaFactor& f, const double (&held)[kMaHeld], float& coef) {
+    const float scale = f.grad_scale_ptr ? (float)((double)*f.grad_scale_ptr * f.grad_scale) : (float)f.grad_scale;
+    coef = scale;
+    if (f.num_partial == 0) return true;
+    const float norm = (float)(sqrt(ma_sum_partials(f.partial, f.num_partial, held)) * fabs((double)scale));
+    if (f.grad_norm && blockIdx.x == 0 && threadIdx.x == 0) *f.grad_norm = norm;
+    if (f.max_norm > 0.f && f.max_norm < INFINITY) {
+        const float c = f.max_norm / (norm + 1e-6f);
+        coef *= c > 1.0f ? 1.0f : c;                                 // NaN stays NaN
+    }
+    return !(f.skip_nonfinite && !(norm < INFINITY));
+}
+
 struct MaPrepareArgs {
     const GeomaeAdamwTensor* rows;
-    const double* partial;
+    const int32_t* chunks;              // [num chunks][2] = (tensor, chunk of that tensor)
     MaScalars* scalars;
-    MaControl* control;
-    float* grad_norm;
-    const float* grad_scale_ptr;
-    double grad_scale, max_norm;
-    int32_t want_norm, num_partial, first_tensor, num_tensors, skip_nonfinite;
+    double* partial;                    // one per norm workgroup of this launch
+    MaFactor factor;                    // skip_nonfinite: decides over the step (no partial sums: nothing to decide yet)
+    float* grad_norm;                   // set where there is no element at all: 0
+    int32_t first_tensor, num_tensors, first_chunk, num_chunks, with_scalars;
     uint32_t seed;
     GeomaeAdamwHyper hypers[kMaHypers];
+    const void* grads[kMaTensors];
     uint8_t hyper_of[kMaTensors];       // 255: no gradient, the tensor is left as it is
 };
 
-// one workgroup: the norm of all tensors from its partial sums (in a fixed order), the factor of the gradients, and what each
-// tensor's update needs of its own step count
+// what each tensor's update needs of its own step count, which it advances
+__device__ __forceinline__ void ma_tensor_scalars(const MaPrepareArgs& a) {
+    double held[kMaHeld];
+    float coef;
+    ma_load_partials(a.factor.partial, a.factor.num_partial, held);
+    if (!ma_factor(a.factor, held, coef)) return;
+    if (a.grad_norm && threadIdx.x == 0) *a.grad_norm = 0.f;
+    for (int t = threadIdx.x; t < a.num_tensors; t += kMaThreads) {
+        if (a.hyper_of[t] == 255) continue;
+        const GeomaeAdamwTensor row = a.rows[a.first_tensor + t];
+        const GeomaeAdamwHyper h = a.hypers[a.hyper_of[t]];
+        const int64_t step = *row.step + 1;
+        *row.step = step;
+        const double lr = h.lr_ptr ? (double)*h.lr_ptr : h.lr;
+        const double bc1 = 1.0 - pow(h.beta1, (double)step), bc2 = 1.0 - pow(h.beta2, (double)step);
+        MaScalars s;
+        s.decay = (float)(1.0 - lr * h.weight_decay);
+        s.w1 = (float)(1.0 - h.beta1);
+        s.b2 = (float)h.beta2;
+        s.omb2 = (float)(1.0 - h.beta2);
+        s.bc2_sqrt = (float)sqrt(bc2);
+        s.inv_bc2_sqrt = (float)(1.0 / sqrt(bc2));
+        s.eps = (float)h.eps;
+        s.step_size = (float)(lr / bc1);
+        s.key = ma_mix(ma_mix(a.seed + 0x9E3779B9u * (uint32_t)row.index) ^ (uint32_t)step);
+        a.scalars[a.first_tensor + t] = s;
+    }
+}
+
+// Workgroup 0: the scalars (two powers in fp64 per tensor: started first, hidden behind the others).  The rest: partial sums of
+// the squares, the next chunk's table entries loaded ahead of this chunk's data (three dependent loads a chunk otherwise).  The
+// update's workgroups add the partial sums themselves, while their own data is on its way: a last workgroup that collects
+// them here has to order its reads behind the others' writes, and the cache write-back of that, once per workgroup, made this
+// launch six times as long (48 M elements: 269 us against 43).
 __global__ __launch_bounds__(kMaThreads) void multi_prepare_kernel(MaPrepareArgs a) {
+    if (a.with_scalars && blockIdx.x == 0) {
+        ma_tensor_scalars(a);
+        return;
+    }
     __shared__ double red[kMaThreads / kWave];
-    __shared__ int32_t skip_s;
+    const int blocks = gridDim.x - a.with_scalars, block = blockIdx.x - a.with_scalars;
     double acc = 0.0;
-    for (int i = threadIdx.x; i < a.num_partial; i += kMaThreads) acc += a.partial[i];
+    const int2* chunks = reinterpret_cast<const int2*>(a.chunks) + a.first_chunk;
+    int2 at = chunks[block];
+    int64_t n = a.rows[at.x].numel;
+    int dtype = a.rows[at.x].dtype;
+    for (int c = block; c < a.num_chunks; c += blocks) {
+        const void* g = a.grads[at.x - a.first_tensor];
+        const int64_t start = (int64_t)at.y * kMaChunk, left = n;
+        const int now = dtype;
+        if (c + blocks < a.num_chunks) {
+            at = chunks[c + blocks];
+            n = a.rows[at.x].numel;
+            dtype = a.rows[at.x].dtype;
+        }
+        if (!g) continue;
+        if (now == GEOMAE_DTYPE_F32) acc += ma_sumsq<float>(g, start, left);
+        else if (now == GEOMAE_DTYPE_BF16) acc += ma_sumsq<uint16_t>(g, start, left);
+        else acc += ma_sumsq<_Float16>(g, start, left);
+    }
     acc = wave_sum(acc);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        const float scale = a.grad_scale_ptr ? (float)((double)*a.grad_scale_ptr * a.grad_scale) : (float)a.grad_scale;
-        float coef = scale;
-        int32_t skip = 0;
-        if (a.want_norm) {
-            const float norm = (float)(sqrt(red[0] + red[1] + red[2] + red[3]) * fabs((double)scale));
-            if (a.grad_norm) *a.grad_norm = norm;
-            if (a.max_norm > 0.0 && a.max_norm < INFINITY) {
-                const float c = (float)a.max_norm / (norm + 1e-6f);
-                coef *= c > 1.0f ? 1.0f : c;                         // NaN stays NaN
-            }
-            skip = a.skip_nonfinite && !(norm < INFINITY);
-        }
-        a.control->coef = coef;
-        a.control->skip = skip;
-        skip_s = skip;
-    }
-    __syncthreads();
-    const int t = threadIdx.x;
-    if (skip_s || t >= a.num_tensors || a.hyper_of[t] == 255) return;
-    const GeomaeAdamwTensor row = a.rows[a.first_tensor + t];
-    const GeomaeAdamwHyper h = a.hypers[a.hyper_of[t]];
-    const int64_t step = *row.step + 1;
-    *row.step = step;
-    const double lr = h.lr_ptr ? (double)*h.lr_ptr : h.lr;
-    const double bc1 = 1.0 - pow(h.beta1, (double)step), bc2 = 1.0 - pow(h.beta2, (double)step);
-    MaScalars s;
-    s.decay = (float)(1.0 - lr * h.weight_decay);
-    s.w1 = (float)(1.0 - h.beta1);
-    s.b2 = (float)h.beta2;
-    s.omb2 = (float)(1.0 - h.beta2);
-    s.bc2_sqrt = (float)sqrt(bc2);
-    s.eps = (float)h.eps;
-    s.step_size = (float)(lr / bc1);
-    s.key = ma_mix(ma_mix(a.seed + 0x9E3779B9u * (uint32_t)row.index) ^ (uint32_t)step);
-    a.scalars[a.first_tensor + t] = s;
+    if (threadIdx.x == 0) a.partial[block] = red[0] + red[1] + red[2] + red[3];
 }
 
 // ------------------------------------------------------------------------------------------------ update
@@ -262,47 +289,59 @@ struct MaStepArgs {
     const GeomaeAdamwTensor* rows;
     const int32_t* chunks;
     const MaScalars* scalars;
-    const MaControl* control;
+    MaFactor factor;
     int32_t first_tensor, first_chunk;
     const void* grads[kMaTensors];
 };
 
-template <typename T, bool MASTER, int BITS>
-__device__ __forceinline__ void ma_update(const GeomaeAdamwTensor& row, const T* g, int64_t start, const MaScalars& s, float coef) {
-    const int64_t n = row.numel, padded = (n + 31) & ~(int64_t)31;   // the moments' and masters' own length
-    T* param = static_cast<T*>(row.param);
+__device__ __forceinline__ float ma_sqrt(float v) {                  // (the instruction takes subnormal numbers for zero)
+    const bool tiny = v < 0x1p-96f;
+    return __builtin_amdgcn_sqrtf(tiny ? v * 0x1p32f : v) * (tiny ? 0x1p-16f : 1.0f);
+}
+
+template <typename T, bool MASTER, int BITS, bool FULL>
+__device__ __forceinline__ void ma_update(const GeomaeAdamwTensor& row, const T* g, int64_t start, int left, const MaScalars& s, const MaFactor& factor) {
+    const int padded = (left + 31) & ~31;                            // the moments' and masters' own length
+    T* param = static_cast<T*>(row.param) + start;
+    float* master = MASTER ? row.master + start : nullptr;
+    float *m32 = static_cast<float*>(row.exp_avg) + start, *v32 = static_cast<float*>(row.exp_avg_sq) + start;
+    uint8_t *m8 = static_cast<uint8_t*>(row.exp_avg) + start, *r8 = static_cast<uint8_t*>(row.exp_avg_sq) + start;
+    uint8_t *me8 = row.exp_avg_exponent + (start >> 5), *re8 = row.exp_avg_sq_exponent + (start >> 5);
     float gv[kMaIters][kMaVec], pv[kMaIters][kMaVec], mv[kMaIters][kMaVec], vv[kMaIters][kMaVec];
     uint32_t mw[kMaIters], rw[kMaIters];
     int me[kMaIters], re[kMaIters];
+    double held[kMaHeld];
+    ma_load_partials(factor.partial, factor.num_partial, held);      // (first: loads complete in order)
 #pragma unroll
     for (int it = 0; it < kMaIters; ++it) {
-        const int64_t e = start + (it * kMaThreads + (int)threadIdx.x) * kMaVec;
-        if (e >= padded) continue;                                   // whole groups of 8 lanes
-        ma_load<T>(g, e < n ? e : n, n, gv[it]);
+        const int o = (it * kMaThreads + (int)threadIdx.x) * kMaVec;
+        if (!FULL && o >= padded) continue;                          // whole groups of 8 lanes
+        ma_load<FULL, T>(g, o, left, gv[it]);
         if constexpr (MASTER) {
-            const float4 w = *reinterpret_cast<const float4*>(row.master + e);
+            const float4 w = *reinterpret_cast<const float4*>(master + o);
             pv[it][0] = w.x; pv[it][1] = w.y; pv[it][2] = w.z; pv[it][3] = w.w;
-        } else ma_load<T>(param, e < n ? e : n, n, pv[it]);
+        } else ma_load<FULL, T>(param, o, left, pv[it]);
         if constexpr (BITS == 32) {
-            const float4 m = *reinterpret_cast<const float4*>(static_cast<const float*>(row.exp_avg) + e);
-            const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(row.exp_avg_sq) + e);
+            const float4 m = *reinterpret_cast<const float4*>(m32 + o), v = *reinterpret_cast<const float4*>(v32 + o);
             mv[it][0] = m.x; mv[it][1] = m.y; mv[it][2] = m.z; mv[it][3] = m.w;
             vv[it][0] = v.x; vv[it][1] = v.y; vv[it][2] = v.z; vv[it][3] = v.w;
         } else {
-            mw[it] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(row.exp_avg) + e);
-            rw[it] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(row.exp_avg_sq) + e);
-            me[it] = row.exp_avg_exponent[e >> 5];
-            re[it] = row.exp_avg_sq_exponent[e >> 5];
+            mw[it] = *reinterpret_cast<const uint32_t*>(m8 + o);
+            rw[it] = *reinterpret_cast<const uint32_t*>(r8 + o);
+            me[it] = me8[o >> 5];
+            re[it] = re8[o >> 5];
         }
     }
+    float coef;
+    if (!ma_factor(factor, held, coef)) return;
 #pragma unroll
     for (int it = 0; it < kMaIters; ++it) {
-        const int64_t e = start + (it * kMaThreads + (int)threadIdx.x) * kMaVec;
-        if (e >= padded) continue;
+        const int o = (it * kMaThreads + (int)threadIdx.x) * kMaVec;
+        if (!FULL && o >= padded) continue;
         float r[kMaVec];
         if constexpr (BITS == 8) {
-            ma_value_signed(mw[it], ma_unscale(me[it]), mv[it]);
-            ma_value_root(rw[it], ma_unscale(re[it]), r);
+            ma_value_signed(mw[it], me[it], mv[it]);
+            ma_value_root(rw[it], re[it], r);
 #pragma unroll
             for (int i = 0; i < kMaVec; ++i) vv[it][i] = __fmul_rn(r[i], r[i]);
         }
@@ -312,35 +351,49 @@ __device__ __forceinline__ void ma_update(const GeomaeAdamwTensor& row, const T*
             float& m = mv[it][i];
             float& v = vv[it][i];
             const float d = __fsub_rn(x, m);
-            m = s.w1 < 0.5f ? __fadd_rn(m, __fmul_rn(s.w1, d)) : __fsub_rn(x, __fmul_rn(d, __fsub_rn(1.0f, s.w1)));
+            if (BITS == 8 || s.w1 < 0.5f) m = __fadd_rn(m, __fmul_rn(s.w1, d));
+            else m = __fsub_rn(x, __fmul_rn(d, __fsub_rn(1.0f, s.w1)));
             v = __fadd_rn(__fmul_rn(v, s.b2), __fmul_rn(__fmul_rn(s.omb2, x), x));
-            r[i] = __fsqrt_rn(v);
-            float p = __fmul_rn(pv[it][i], s.decay);
-            const float denom = __fadd_rn(__fdiv_rn(r[i], s.bc2_sqrt), s.eps);
-            pv[it][i] = __fadd_rn(p, __fmul_rn(-s.step_size, __fdiv_rn(m, denom)));
+            const float p = __fmul_rn(pv[it][i], s.decay);
+            if constexpr (BITS == 32) {                              // torch.optim.AdamW's roundings; HBM hides them
+                const float denom = __fadd_rn(__fdiv_rn(__fsqrt_rn(v), s.bc2_sqrt), s.eps);
+                pv[it][i] = __fadd_rn(p, __fmul_rn(-s.step_size, __fdiv_rn(m, denom)));
+            } else {                                                 // half the bytes: the hardware's 1-ulp root and reciprocal
+                r[i] = ma_sqrt(v);
+                pv[it][i] = __fadd_rn(p, __fmul_rn(-s.step_size, m * __builtin_amdgcn_rcpf(__fadd_rn(r[i] * s.inv_bc2_sqrt, s.eps))));
+            }
         }
-        if (e < n) ma_store<T>(param, e, n, pv[it]);
+        ma_store<FULL, T>(param, o, left, pv[it]);
         if constexpr (MASTER) {
+            if constexpr (!FULL) {
 #pragma unroll
-            for (int i = 0; i < kMaVec; ++i) pv[it][i] = e + i < n ? pv[it][i] : 0.f;             // (0 / 0 where eps is 0)
-            *reinterpret_cast<float4*>(row.master + e) = make_float4(pv[it][0], pv[it][1], pv[it][2], pv[it][3]);
+                for (int i = 0; i < kMaVec; ++i) pv[it][i] = o + i < left ? pv[it][i] : 0.f;         // (0 / 0 where eps is 0)
+            }
+            *reinterpret_cast<float4*>(master + o) = make_float4(pv[it][0], pv[it][1], pv[it][2], pv[it][3]);
         }
         if constexpr (BITS == 32) {
-            *reinterpret_cast<float4*>(static_cast<float*>(row.exp_avg) + e) = make_float4(mv[it][0], mv[it][1], mv[it][2], mv[it][3]);
-            *reinterpret_cast<float4*>(static_cast<float*>(row.exp_avg_sq) + e) = make_float4(vv[it][0], vv[it][1], vv[it][2], vv[it][3]);
+            *reinterpret_cast<float4*>(m32 + o) = make_float4(mv[it][0], mv[it][1], mv[it][2], mv[it][3]);
+            *reinterpret_cast<float4*>(v32 + o) = make_float4(vv[it][0], vv[it][1], vv[it][2], vv[it][3]);
         } else {
+            const uint32_t first = s.key + (uint32_t)start + (uint32_t)o;
             uint32_t draw[kMaVec];
 #pragma unroll
-            for (int i = 0; i < kMaVec; ++i) draw[i] = ma_mix(s.key + (uint32_t)(e + i));
+            for (int i = 0; i < kMaVec; ++i) draw[i] = ma_mix(first + (uint32_t)i);
             const int em = ma_exponent<true>(ma_block_max(mv[it])), er = ma_exponent<false>(ma_block_max(r));
-            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(row.exp_avg) + e) = ma_code_signed(mv[it], ma_scale(em), draw);
-            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(row.exp_avg_sq) + e) = ma_code_root(r, ma_scale(er), draw);
+            *reinterpret_cast<uint32_t*>(m8 + o) = ma_code_signed(mv[it], ma_scale(em), draw);
+            *reinterpret_cast<uint32_t*>(r8 + o) = ma_code_root(r, ma_scale(er), draw);
             if ((threadIdx.x & 7) == 0) {
-                row.exp_avg_exponent[e >> 5] = (uint8_t)em;
-                row.exp_avg_sq_exponent[e >> 5] = (uint8_t)er;
+                me8[o >> 5] = (uint8_t)em;
+                re8[o >> 5] = (uint8_t)er;
             }
         }
     }
+}
+template <typename T, bool MASTER, int BITS>
+__device__ __forceinline__ void ma_update(const GeomaeAdamwTensor& row, const void* g, int64_t start, const MaScalars& s, const MaFactor& factor) {
+    const T* p = static_cast<const T*>(g) + start;
+    if (row.numel - start >= kMaChunk) ma_update<T, MASTER, BITS, true>(row, p, start, kMaChunk, s, factor);
+    else ma_update<T, MASTER, BITS, false>(row, p, start, (int)(row.numel - start), s, factor);
 }
 
 template <int BITS>
@@ -349,17 +402,24 @@ __global__ __launch_bounds__(kMaThreads) void multi_adamw_kernel(MaStepArgs a) {
     const int t = at[0];
     const int64_t start = (int64_t)at[1] * kMaChunk;
     const void* g = a.grads[t - a.first_tensor];
-    if (!g || a.control->skip) return;
-    const float coef = a.control->coef;
+    if (!g) {
+        // (it may be the one that writes the norm)
+        double held[kMaHeld];
+        float coef;
+        if (!(a.factor.grad_norm && blockIdx.x == 0)) return;
+        ma_load_partials(a.factor.partial, a.factor.num_partial, held);
+        ma_factor(a.factor, held, coef);
+        return;
+    }
     const GeomaeAdamwTensor row = a.rows[t];
     const MaScalars s = a.scalars[t];
-    if (row.dtype == GEOMAE_DTYPE_F32) ma_update<float, false, BITS>(row, static_cast<const float*>(g), start, s, coef);
+    if (row.dtype == GEOMAE_DTYPE_F32) ma_update<float, false, BITS>(row, g, start, s, a.factor);
     else if (row.dtype == GEOMAE_DTYPE_BF16) {
-        if (row.master) ma_update<uint16_t, true, BITS>(row, static_cast<const uint16_t*>(g), start, s, coef);
-        else ma_update<uint16_t, false, BITS>(row, static_cast<const uint16_t*>(g), start, s, coef);
+        if (row.master) ma_update<uint16_t, true, BITS>(row, g, start, s, a.factor);
+        else ma_update<uint16_t, false, BITS>(row, g, start, s, a.factor);
     } else {
-        if (row.master) ma_update<_Float16, true, BITS>(row, static_cast<const _Float16*>(g), start, s, coef);
-        else ma_update<_Float16, false, BITS>(row, static_cast<const _Float16*>(g), start, s, coef);
+        if (row.master) ma_update<_Float16, true, BITS>(row, g, start, s, a.factor);
+        else ma_update<_Float16, false, BITS>(row, g, start, s, a.factor);
     }
 }
 
@@ -374,24 +434,23 @@ __global__ __launch_bounds__(256) void adamw_moments8_kernel(const uint32_t* m, 
     };
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
         float x[kMaVec];
-        ma_value_signed(m[i], ma_unscale(me[i >> 3]), x);
+        ma_value_signed(m[i], me[i >> 3], x);
         put(m_out, i, x);
-        ma_value_root(r[i], ma_unscale(re[i >> 3]), x);
+        ma_value_root(r[i], re[i >> 3], x);
         put(r_out, i, x);
     }
 }
 
-struct MaWorkspace { double* partial; MaScalars* scalars; MaControl* control; int64_t bytes; };
+static_assert(sizeof(MaPrepareArgs) <= 4096 && sizeof(MaStepArgs) <= 4096, "a launch takes 4 KB of arguments");
+struct MaWorkspace { double* partial; MaScalars* scalars; int64_t bytes; };
 static MaWorkspace ma_workspace(void* base, int32_t num_tensors) {
-    const int64_t slices = (num_tensors + kMaTensors - 1) / kMaTensors;
     char* p = static_cast<char*>(base);
     MaWorkspace w;
+    // a launch of few tensors (one for every kMaHypers hyper-parameter sets at worst) has one norm workgroup at least
+    const int64_t partial = (kMaNormGrid + (int64_t)num_tensors) * (int64_t)sizeof(double);
     w.partial = reinterpret_cast<double*>(p);
-    const int64_t scal = slices * kMaNormGrid * (int64_t)sizeof(double);
-    w.scalars = reinterpret_cast<MaScalars*>(p + scal);
-    const int64_t ctl = scal + (int64_t)num_tensors * (int64_t)sizeof(MaScalars);
-    w.control = reinterpret_cast<MaControl*>(p + ctl);
-    w.bytes = ctl + 256;
+    w.scalars = reinterpret_cast<MaScalars*>(p + partial);
+    w.bytes = partial + (int64_t)num_tensors * (int64_t)sizeof(MaScalars);
     return w;
 }
 
@@ -424,33 +483,12 @@ extern "C" int geomae_multi_adamw_step(const GeomaeAdamwTensor* table, const int
         GEOMAE_REQUIRE(!grads[t] || (hyper_of[t] >= 0 && hyper_of[t] < num_hypers), "multi_adamw_step: hyper-parameter set %d of tensor %d out of range",
                        (int)hyper_of[t], (int)t);
     }
-    const bool norm = max_norm > 0.0 || skip_nonfinite || grad_norm_out;
-    int32_t num_partial = 0;
-    if (norm) {
-        MaNormArgs a;
-        a.rows = table; a.chunks = chunks;
-        for (int32_t t0 = 0; t0 < num_tensors; t0 += kMaTensors) {
-            const int32_t t1 = t0 + kMaTensors < num_tensors ? t0 + kMaTensors : num_tensors;
-            a.first_tensor = t0; a.first_chunk = (int32_t)first_chunk[t0]; a.num_chunks = (int32_t)(first_chunk[t1] - first_chunk[t0]);
-            if (a.num_chunks == 0) continue;
-            for (int32_t t = t0; t < t1; ++t) a.grads[t - t0] = grads[t];
-            const int grid = a.num_chunks < kMaNormGrid ? a.num_chunks : kMaNormGrid;
-            a.partial = w.partial + num_partial;
-            hipLaunchKernelGGL(multi_sumsq_kernel, dim3(grid), dim3(kMaThreads), 0, stream, a);
-            num_partial += grid;
-        }
-        if (int rc = check_launch("multi_sumsq_kernel")) return rc;
-    }
+    // slices of at most kMaTensors tensors and kMaHypers distinct hyper-parameter sets
     MaPrepareArgs pa;
-    pa.rows = table; pa.partial = w.partial; pa.scalars = w.scalars; pa.control = w.control;
-    pa.grad_norm = grad_norm_out; pa.grad_scale_ptr = grad_scale_ptr; pa.grad_scale = grad_scale; pa.max_norm = max_norm;
-    pa.want_norm = norm; pa.num_partial = num_partial; pa.skip_nonfinite = skip_nonfinite; pa.seed = seed;
-    MaStepArgs sa;
-    sa.rows = table; sa.chunks = chunks; sa.scalars = w.scalars; sa.control = w.control;
-    for (int32_t t0 = 0; t0 < num_tensors;) {        // slices of at most kMaTensors tensors and kMaHypers distinct hyper-parameter sets
+    auto slice = [&](int32_t t0) {
         int32_t slot_of[kMaHypers], used = 0, t = t0;
         for (; t < num_tensors && t - t0 < kMaTensors; ++t) {
-            sa.grads[t - t0] = grads[t];
+            pa.grads[t - t0] = grads[t];
             pa.hyper_of[t - t0] = 255;
             if (!grads[t]) continue;
             int32_t k = 0;
@@ -462,15 +500,53 @@ extern "C" int geomae_multi_adamw_step(const GeomaeAdamwTensor* table, const int
             }
             pa.hyper_of[t - t0] = (uint8_t)k;
         }
-        pa.first_tensor = t0; pa.num_tensors = t - t0;
+        pa.first_tensor = t0;
+        pa.num_tensors = t - t0;
+        pa.first_chunk = (int32_t)first_chunk[t0];
+        pa.num_chunks = (int32_t)(first_chunk[t] - first_chunk[t0]);
+        return t;
+    };
+    const int64_t chunks_all = first_chunk[num_tensors];
+    const bool norm = (max_norm > 0.0 || skip_nonfinite || grad_norm_out) && chunks_all > 0;
+    pa.rows = table; pa.chunks = chunks; pa.scalars = w.scalars; pa.seed = seed;
+    pa.factor = {w.partial, 0, skip_nonfinite, grad_scale, grad_scale_ptr, (float)max_norm, nullptr};
+    pa.grad_norm = chunks_all == 0 ? grad_norm_out : nullptr;
+    int32_t num_partial = 0;
+    // skip_nonfinite: the scalars wait for the whole norm, a launch of their own
+    for (int pass = 0; pass < 2; ++pass) {
+        if (pass == 1 && !(norm && skip_nonfinite)) break;
+        pa.with_scalars = !(norm && skip_nonfinite) || pass == 1;
+        pa.factor.num_partial = pass == 1 ? num_partial : 0;
+        for (int32_t t0 = 0; t0 < num_tensors;) {
+            const int32_t t1 = slice(t0);
+            int grid = 0;
+            if (norm && pass == 0 && pa.num_chunks > 0) {            // a share of kMaNormGrid by size
+                grid = (int)((int64_t)kMaNormGrid * pa.num_chunks / chunks_all);
+                grid = grid < 1 ? 1 : (grid > pa.num_chunks ? pa.num_chunks : grid);
+            }
+            pa.partial = w.partial + num_partial;
+            num_partial += grid;
+            if (grid + pa.with_scalars > 0)
+                hipLaunchKernelGGL(multi_prepare_kernel, dim3(grid + pa.with_scalars), dim3(kMaThreads), 0, stream, pa);
+            t0 = t1;
+        }
+    }
+    MaStepArgs sa;
+    sa.rows = table; sa.chunks = chunks; sa.scalars = w.scalars;
+    sa.factor = pa.factor;
+    sa.factor.num_partial = num_partial;
+    sa.factor.grad_norm = grad_norm_out;
+    for (int32_t t0 = 0; t0 < num_tensors;) {
+        const int32_t t1 = t0 + kMaTensors < num_tensors ? t0 + kMaTensors : num_tensors;
+        for (int32_t t = t0; t < t1; ++t) sa.grads[t - t0] = grads[t];
         sa.first_tensor = t0; sa.first_chunk = (int32_t)first_chunk[t0];
-        const int64_t num_chunks = first_chunk[t] - first_chunk[t0];
-        hipLaunchKernelGGL(multi_prepare_kernel, dim3(1), dim3(kMaThreads), 0, stream, pa);
+        const int64_t num_chunks = first_chunk[t1] - first_chunk[t0];
         if (num_chunks > 0) {
             if (state_bits == 32) hipLaunchKernelGGL(multi_adamw_kernel<32>, dim3((uint32_t)num_chunks), dim3(kMaThreads), 0, stream, sa);
             else hipLaunchKernelGGL(multi_adamw_kernel<8>, dim3((uint32_t)num_chunks), dim3(kMaThreads), 0, stream, sa);
+            sa.factor.grad_norm = nullptr;
         }
-        t0 = t;
+        t0 = t1;
     }
     return check_launch("multi_adamw_kernel");
 }
