@@ -1,4 +1,4 @@
-// Group norm with an activation on channels-last data: x [n][rows][c], groups of c / groups neighbouring channels.
+// Group norm with an activation on channels-last data: x [n][rows][c], groups of cg = c / groups neighbouring channels.
 //
 //   xhat = (x - mean) rstd,  z = gamma xhat + beta,  y = act(z)        mean, var over the rows and channels of (sample, group)
 //   dz = dy act'(z);  dbeta = sum dz, dgamma = sum dz xhat over samples and rows
@@ -10,10 +10,13 @@
 // true one.  The rest is fp32; the gradient sums are fp32 within a workgroup's rows and fp64 across workgroups, always in the
 // same order.
 //
-// What bounds it: HBM, and the launches at small sizes.  Three launches each way: sums over a chunk of rows, one value per
-// (sample, group) from the chunks' sums, and the pass that writes.  The second read of x (and dy) comes from the 256 MB cache
-// where the tensors fit in it.  A thread keeps to one vector of neighbouring channels, so that its gamma, beta and statistics
-// stay in registers, and a workgroup's accesses cover whole rows, contiguous in memory.
+// A thread keeps to one vector of V neighbouring channels of one group (V the largest power of two up to 16 bytes that divides
+// cg; up to 4 where x and dy are both held), so that its statistics, gamma and beta stay in registers.  Two forms:
+//  resident  all rows of one or more groups fit a workgroup's registers (128 bytes a thread, 1024 threads: 4096 rows of 32
+//            bytes): x and dy are read once and one launch does a pass (the backward pass one more for the parameters'
+//            gradients if there is more than one sample).  Bound by launch, load latency and the workgroup's reductions.
+//  streamed  three launches a pass: sums over a chunk of rows, one value per (sample, group) from the chunks' sums, and the pass
+//            that writes.  Bound by HBM, or the 256 MB cache that the second read of x and dy comes from where they fit in it.
 #include "common.h"
 #include "../../include/geomae_hip.h"
 #include <math.h>
@@ -21,46 +24,93 @@
 
 namespace geomae {
 
-constexpr int kGnThreads = 256;
-constexpr int kGnUnroll = 4;                       // rows in flight per thread
+constexpr int kGnThreads = 256;                    // of a streamed workgroup
 constexpr int kGnMaxGroups = 1024;
-constexpr int kGnBlocks = 1024;                    // workgroups of a pass: four per CU
+constexpr int kGnBlocks = 1024;                    // workgroups of a streamed pass: four per CU
 constexpr int kGnFold = 64;                        // samples whose sums one thread adds up for the parameters' gradients
+constexpr int kGnResidentThreads = 1024;
 
 enum { kGnNone = 0, kGnRelu = 1, kGnSilu = 2, kGnGelu = 3 };
 
 struct GnShape {
     int64_t rows;                                  // of a sample
     int32_t n, c, groups, cg;
-    int32_t chunks;                                // of a sample's rows
+    int32_t chunks;                                // of a sample's rows (streamed)
     int64_t chunk_rows;
+    int32_t v;                                     // channels of a thread
+    int32_t cs, threads;                           // channels of a resident workgroup, 0: streamed; its threads
 };
 
 template <typename T> __device__ __forceinline__ float gn_float(T x) { return (float)x; }
 template <> __device__ __forceinline__ float gn_float<uint16_t>(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }   // bf16
-template <typename T> __device__ __forceinline__ T gn_narrow(float x) { return (T)x; }
-template <> __device__ __forceinline__ uint16_t gn_narrow<uint16_t>(float x) {
-    const uint32_t b = __float_as_uint(x);
-    return x != x ? (uint16_t)((b >> 16) | 0x40) : (uint16_t)((b + 0x7fff + ((b >> 16) & 1)) >> 16);
-}
 // (element-aligned: a tensor may start anywhere, and global memory takes wide accesses at any element's address)
 template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) GnPack { T v[V]; };
 template <typename T, int V> __device__ __forceinline__ GnPack<T, V> gn_read(const T* p) { return *reinterpret_cast<const GnPack<T, V>*>(p); }
+typedef __bf16 GnBf2 __attribute__((ext_vector_type(2)));
+typedef float GnF2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t gn_bf16_pair(float a, float b) {
+    const GnBf2 r = __builtin_convertvector((GnF2){a, b}, GnBf2);
+    return __builtin_bit_cast(uint32_t, r);
+}
+template <typename T, int V> __device__ __forceinline__ void gn_write(T* p, const float (&x)[V]) {
+    GnPack<T, V> w;
+    if constexpr (std::is_same<T, uint16_t>::value) {
+#pragma unroll
+        for (int i = 0; i + 1 < V; i += 2) {
+            const uint32_t two = gn_bf16_pair(x[i], x[i + 1]);
+            w.v[i] = (uint16_t)two;
+            w.v[i + 1] = (uint16_t)(two >> 16);
+        }
+        if constexpr (V == 1) w.v[0] = (uint16_t)gn_bf16_pair(x[0], 0.f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w.v[i] = (T)x[i];
+    }
+    *reinterpret_cast<GnPack<T, V>*>(p) = w;
+}
+// vectors that a thread has in flight (streamed; 64 bytes) or holds (resident)
+template <typename T, int V> constexpr int gn_unroll() { return 64 / (int)(V * sizeof(T)) < 16 ? 64 / (int)(V * sizeof(T)) : 16; }
+template <typename T, int V> constexpr int gn_held() { return V * sizeof(T) == 16 ? 8 : 16; }
+static int gn_vectors_held(int v, int item) { return v * item == 16 ? 8 : 16; }
 
+// The hardware's base-2 exponential and reciprocal (1 ulp each): the library's expf and the IEEE division made silu and gelu, not
+// memory, the bound (61 M bf16 elements, silu: 85 us).  erf by Abramowitz and Stegun 7.1.26 (off by 1.5e-7 at most, which is
+// 1.3 units of fp32's rounding at 1), whose exponential is also the density of gelu's slope.
+__device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f)); }
+__device__ __forceinline__ float gn_normal_cdf(float z, float& density) {       // density: exp(-z^2 / 2)
+    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+    density = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+    const float poly = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
+    const float tail = 0.5f * (poly * t) * density;
+    return z < 0.f ? tail : 1.0f - tail;
+}
 template <int ACT> __device__ __forceinline__ float gn_act(float z) {
     if constexpr (ACT == kGnRelu) return z < 0.f ? 0.f : z;            // NaN stays
-    if constexpr (ACT == kGnSilu) return z / (1.0f + expf(-z));
-    if constexpr (ACT == kGnGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    if constexpr (ACT == kGnSilu) return z * gn_sigmoid(z);
+    if constexpr (ACT == kGnGelu) {
+        float density;
+        return z * gn_normal_cdf(z, density);
+    }
     return z;
 }
 template <int ACT> __device__ __forceinline__ float gn_slope(float z) {     // (ReLU's: gn_threshold)
     if constexpr (ACT == kGnSilu) {
-        const float s = 1.0f / (1.0f + expf(-z));
-        return s * (1.0f + z * (1.0f - s));
+        const float s = gn_sigmoid(z);
+        return s * fmaf(z, 1.0f - s, 1.0f);
     }
-    if constexpr (ACT == kGnGelu)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    if constexpr (ACT == kGnGelu) {
+        float density;
+        const float cdf = gn_normal_cdf(z, density);
+        return fmaf(z * 0.39894228040143268f, density, cdf);
+    }
     return 1.0f;
+}
+// f(activation), the run-time choice made outside the loops
+template <typename F> __host__ __device__ __forceinline__ void gn_by_act(int act, F f) {
+    if (act == kGnRelu) f(std::integral_constant<int, kGnRelu>());
+    else if (act == kGnSilu) f(std::integral_constant<int, kGnSilu>());
+    else if (act == kGnGelu) f(std::integral_constant<int, kGnGelu>());
+    else f(std::integral_constant<int, kGnNone>());
 }
 // z > 0 as a comparison of sign * x with a threshold
 __device__ __forceinline__ void gn_threshold(double mean, double scale, double beta, float& sign, float& thr) {
@@ -81,9 +131,292 @@ __device__ __forceinline__ float gn_weight(const void* w, int dtype, int c, floa
     if (dtype == GEOMAE_DTYPE_BF16) return gn_float(static_cast<const uint16_t*>(w)[c]);
     return gn_float(static_cast<const _Float16*>(w)[c]);
 }
+__device__ __forceinline__ void gn_store_weight(void* w, int dtype, int c, float v) {
+    if (!w) return;
+    if (dtype == GEOMAE_DTYPE_F32) static_cast<float*>(w)[c] = v;
+    else if (dtype == GEOMAE_DTYPE_BF16) static_cast<uint16_t*>(w)[c] = (uint16_t)gn_bf16_pair(v, 0.f);
+    else static_cast<_Float16*>(w)[c] = (_Float16)v;
+}
 
-// ------------------------------------------------------------------------------------------------ sums of x
-// the workgroup's lanes as tx columns (vectors of V channels) x ty rows; c > 256 V is walked in tiles of 256 V channels
+struct GnWeights { const void *gamma, *beta; int dtype; };
+
+// what a lane keeps of its V channels, all of one group, for y
+template <int V> struct GnScale {
+    float mean, scale[V], rest[V], beta[V];
+    __device__ __forceinline__ void load(double2 stat, const GnWeights& w, int col) {
+        mean = (float)stat.x;
+        const double lost = stat.x - (double)mean;                     // what mean's rounding lost comes back behind the product
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const double sc = stat.y * (double)gn_weight(w.gamma, w.dtype, col + i, 1.f);
+            scale[i] = (float)sc;
+            rest[i] = (float)(-lost * sc);
+            beta[i] = gn_weight(w.beta, w.dtype, col + i, 0.f);
+        }
+    }
+    template <int ACT> __device__ __forceinline__ float value(int i, float x) const { return gn_act<ACT>(fmaf(x - mean, scale[i], rest[i]) + beta[i]); }
+};
+// ... and for xhat and dz
+template <int V> struct GnGrad {
+    float mean, rstd, rest, gamma[V], beta[V], sign[V], thr[V];
+    __device__ __forceinline__ void load(double2 stat, const GnWeights& w, int act, int col) {
+        mean = (float)stat.x;
+        rstd = (float)stat.y;
+        rest = (float)(-(stat.x - (double)mean) * stat.y);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            gamma[i] = gn_weight(w.gamma, w.dtype, col + i, 1.f);
+            beta[i] = gn_weight(w.beta, w.dtype, col + i, 0.f);
+            if (act == kGnRelu) gn_threshold(stat.x, stat.y * (double)gamma[i], (double)beta[i], sign[i], thr[i]);
+        }
+    }
+    template <int ACT> __device__ __forceinline__ void value(int i, float x, float dy, float& xhat, float& dz) const {
+        xhat = fmaf(x - mean, rstd, rest);
+        if constexpr (ACT == kGnRelu) dz = x * sign[i] > thr[i] ? dy : 0.f;
+        else dz = dy * gn_slope<ACT>(fmaf(xhat, gamma[i], beta[i]));
+    }
+    // c1, c2: rstd times the group's two means
+    __device__ __forceinline__ float dx(int i, float xhat, float dz, float c1, float c2) const {
+        return fmaf(rstd * gamma[i], dz, -fmaf(xhat, c2, c1));
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ sums over a workgroup
+// a[W] of every thread (row, col) of tx columns x ty rows, summed over the rows: res[w * tx + col].  Fixed order.
+__device__ __forceinline__ bool gn_in_waves(int tx) { return tx <= kWave / 2 && (tx & (tx - 1)) == 0; }
+template <typename S, int W>
+__device__ __forceinline__ void gn_sum_rows(S (&a)[W], int tx, int ty, int row, S* res, S* lds) {
+    const int threads = blockDim.x, t = threadIdx.x;
+    if (gn_in_waves(tx)) {                                             // a wave holds whole rows: its rows first, then the waves
+        const int waves = threads / kWave;
+        for (int o = tx; o < kWave; o <<= 1) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) a[w] += __shfl_xor(a[w], o, kWave);
+        }
+        if (lane_id() < tx) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) lds[(w * waves + t / kWave) * tx + lane_id()] = a[w];
+        }
+        __syncthreads();
+        for (int k = t; k < W * tx; k += threads) {
+            const int w = k / tx, col = k - w * tx;
+            S sum = lds[(w * waves) * tx + col];
+            for (int v = 1; v < waves; ++v) sum += lds[(w * waves + v) * tx + col];
+            res[k] = sum;
+        }
+    } else {
+#pragma unroll
+        for (int w = 0; w < W; ++w) lds[w * threads + t] = a[w];
+        for (int have = ty; have > 1;) {
+            const int half = (have + 1) >> 1;
+            __syncthreads();
+            if (row + half < have) {
+#pragma unroll
+                for (int w = 0; w < W; ++w) lds[w * threads + t] += lds[w * threads + t + half * tx];
+            }
+            have = half;
+        }
+        __syncthreads();
+        if (t < tx) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) res[w * tx + t] = lds[w * threads + t];
+        }
+    }
+    __syncthreads();
+}
+// f(group, b, e, lane, lanes): the entries [b, e) of each of `groups` groups (per of them a group) to be summed by `lanes`
+// neighbouring threads; few entries: a thread a group, else a wave
+template <typename F> __device__ __forceinline__ void gn_each_group(int groups, int per, F f) {
+    if (per <= 16) {
+        for (int g = threadIdx.x; g < groups; g += blockDim.x) f(g, 0, 1);
+    } else {
+        for (int g = threadIdx.x / kWave; g < groups; g += blockDim.x / kWave) f(g, lane_id(), kWave);
+    }
+}
+__device__ __forceinline__ double gn_lanes_sum(double v, int lanes) { return lanes == 1 ? v : wave_sum(v); }
+
+__device__ __forceinline__ double2 gn_statistics(double sum, double sq, double m, double eps) {
+    const double mean = sum / m;
+    double var = sq / m - mean * mean;
+    var = var < 0.0 ? 0.0 : var;                                       // (NaN stays)
+    return make_double2(mean, 1.0 / sqrt(var + eps));
+}
+
+// ------------------------------------------------------------------------------------------------ resident
+// Workgroup -> (sample, first channel): neighbours in memory go to one XCD (workgroup b runs on XCD b mod 8), whose L2 then
+// serves the lines that the channel ranges share.
+__device__ __forceinline__ int gn_spread(int b, int total) {
+    const int each = total / 8, more = total - each * 8, x = b & 7;
+    return x * each + (x < more ? x : more) + (b >> 3);
+}
+struct GnSlab {
+    int tx, ty, row, col;                          // col: this thread's first channel within the slab
+    int n, c0, groups;
+    bool live;
+    template <int V> __device__ __forceinline__ void set(const GnShape& s) {
+        const int slabs = s.c / s.cs, b = gn_spread(blockIdx.x, gridDim.x);
+        n = b / slabs;
+        c0 = (b - n * slabs) * s.cs;
+        groups = s.cs / s.cg;
+        tx = s.cs / V;
+        ty = blockDim.x / tx;
+        row = threadIdx.x / tx;
+        col = (threadIdx.x - row * tx) * V;
+        live = row < ty;
+    }
+};
+extern __shared__ __align__(16) char gn_lds[];
+
+template <typename T, int V>
+__global__ __launch_bounds__(kGnResidentThreads) void gn_resident_forward_kernel(const T* __restrict__ x, GnShape s, GnWeights w, double eps, int act,
+                                                                                T* __restrict__ y, double2* __restrict__ stats) {
+    constexpr int R = gn_held<T, V>();
+    GnSlab l;
+    l.set<V>(s);
+    double2* group = reinterpret_cast<double2*>(gn_lds);
+    double* res = reinterpret_cast<double*>(group + l.groups);
+    double* lds = res + 2 * l.tx;
+    const int64_t base = (int64_t)l.n * s.rows * s.c + l.c0 + l.col;
+    const int rows = (int)s.rows;
+    GnPack<T, V> v[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const int r = l.row + u * l.ty;
+        if (l.live && r < rows) v[u] = gn_read<T, V>(x + base + (int64_t)r * s.c);
+    }
+    double a[2] = {0.0, 0.0};
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (l.live && l.row + u * l.ty < rows) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double d = (double)gn_float(v[u].v[i]);
+                a[0] += d;
+                a[1] = fma(d, d, a[1]);
+            }
+        }
+    gn_sum_rows<double, 2>(a, l.tx, l.ty, l.row, res, lds);
+    const int per = s.cg / V;
+    gn_each_group(l.groups, per, [&](int g, int lane, int lanes) {
+        double sum = 0.0, sq = 0.0;
+        for (int k = lane; k < per; k += lanes) {
+            sum += res[g * per + k];
+            sq += res[l.tx + g * per + k];
+        }
+        sum = gn_lanes_sum(sum, lanes);
+        sq = gn_lanes_sum(sq, lanes);
+        if (lane == 0) {
+            group[g] = gn_statistics(sum, sq, (double)s.rows * s.cg, eps);
+            stats[(int64_t)l.n * s.groups + l.c0 / s.cg + g] = group[g];
+        }
+    });
+    __syncthreads();
+    if (!l.live) return;
+    GnScale<V> ch;
+    ch.load(group[l.col / s.cg], w, l.c0 + l.col);
+    gn_by_act(act, [&](auto A) {
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const int r = l.row + u * l.ty;
+            if (r < rows) {
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = ch.template value<decltype(A)::value>(i, gn_float(v[u].v[i]));
+                gn_write<T, V>(y + base + (int64_t)r * s.c, o);
+            }
+        }
+    });
+}
+
+// channel [n][c] receives the samples' (sum dz, sum dz xhat); one sample: dgamma, dbeta themselves
+template <typename T, int V>
+__global__ __launch_bounds__(kGnResidentThreads) void gn_resident_backward_kernel(const T* __restrict__ x, const T* __restrict__ dy, GnShape s,
+                                                                                 const double2* __restrict__ stats, GnWeights w, int act,
+                                                                                 T* __restrict__ dx, double2* __restrict__ channel, void* dgamma, void* dbeta) {
+    constexpr int R = gn_held<T, V>();
+    GnSlab l;
+    l.set<V>(s);
+    float2* group = reinterpret_cast<float2*>(gn_lds);
+    float* res = reinterpret_cast<float*>(group + l.groups);           // [2 V][tx]
+    float* lds = res + 2 * V * l.tx;
+    const int64_t base = (int64_t)l.n * s.rows * s.c + l.c0 + l.col;
+    const int rows = (int)s.rows;
+    GnPack<T, V> v[R], d[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const int r = l.row + u * l.ty;
+        if (l.live && r < rows) {
+            v[u] = gn_read<T, V>(x + base + (int64_t)r * s.c);
+            d[u] = gn_read<T, V>(dy + base + (int64_t)r * s.c);
+        }
+    }
+    GnGrad<V> ch;
+    const int mine = l.live ? l.col : 0;
+    ch.load(stats[(int64_t)l.n * s.groups + (l.c0 + mine) / s.cg], w, act, l.c0 + mine);
+    float a[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] = b[i] = 0.f;
+    gn_by_act(act, [&](auto A) {
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+            if (l.live && l.row + u * l.ty < rows) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float xhat, dz;
+                    ch.template value<decltype(A)::value>(i, gn_float(v[u].v[i]), gn_float(d[u].v[i]), xhat, dz);
+                    a[i] += dz;
+                    b[i] = fmaf(dz, xhat, b[i]);
+                }
+            }
+    });
+    gn_sum_rows<float, V>(a, l.tx, l.ty, l.row, res, lds);
+    gn_sum_rows<float, V>(b, l.tx, l.ty, l.row, res + V * l.tx, lds);
+    for (int c = threadIdx.x; c < s.cs; c += blockDim.x) {
+        const int k = c / V, i = c - k * V;
+        const float sa = res[i * l.tx + k], sb = res[(V + i) * l.tx + k];
+        if (channel) channel[(int64_t)l.n * s.c + l.c0 + c] = make_double2((double)sa, (double)sb);
+        else {
+            gn_store_weight(dbeta, w.dtype, l.c0 + c, sa);
+            gn_store_weight(dgamma, w.dtype, l.c0 + c, sb);
+        }
+    }
+    gn_each_group(l.groups, s.cg, [&](int g, int lane, int lanes) {
+        double s1 = 0.0, s2 = 0.0;
+        for (int c = g * s.cg + lane; c < (g + 1) * s.cg; c += lanes) {
+            const int k = c / V, i = c - k * V;
+            const double gm = (double)gn_weight(w.gamma, w.dtype, l.c0 + c, 1.f);
+            s1 += gm * (double)res[i * l.tx + k];
+            s2 += gm * (double)res[(V + i) * l.tx + k];
+        }
+        s1 = gn_lanes_sum(s1, lanes);
+        s2 = gn_lanes_sum(s2, lanes);
+        const double m = (double)s.rows * s.cg;
+        if (lane == 0) group[g] = make_float2((float)(s1 / m), (float)(s2 / m));
+    });
+    __syncthreads();
+    if (!l.live) return;
+    const float2 mean = group[l.col / s.cg];
+    const float c1 = ch.rstd * mean.x, c2 = ch.rstd * mean.y;
+    gn_by_act(act, [&](auto A) {
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const int r = l.row + u * l.ty;
+            if (r < rows) {
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float xhat, dz;
+                    ch.template value<decltype(A)::value>(i, gn_float(v[u].v[i]), gn_float(d[u].v[i]), xhat, dz);
+                    o[i] = ch.dx(i, xhat, dz, c1, c2);
+                }
+                gn_write<T, V>(dx + base + (int64_t)r * s.c, o);
+            }
+        }
+    });
+}
+
+// ------------------------------------------------------------------------------------------------ streamed
+// the workgroup's threads as tx columns (vectors of V channels) x ty rows; c > 256 V is walked in tiles of 256 V channels
 struct GnLanes {
     int tx, ty, col, row;
     bool live;
@@ -98,29 +431,24 @@ template <int V> __device__ __forceinline__ GnLanes gn_lanes(int c, int tile) {
     l.live = l.row < l.ty;
     return l;
 }
-
-// a[2 V] of every lane summed over the lanes of its column into slot (column) of the LDS array; fixed order
-template <typename S, int W>
-__device__ __forceinline__ void gn_sum_rows(S (&a)[W], const GnLanes& l, S* lds) {
-    __syncthreads();
+// f(vectors of up to U rows, how many): the lane's rows of [r0, r1), U loads at a time
+template <typename T, int V, int U, typename F> __device__ __forceinline__ void gn_rows(const T* x, int c, const GnLanes& l, int64_t r0, int64_t r1, F f) {
+    for (int64_t r = r0 + l.row; r < r1; r += U * l.ty) {
+        GnPack<T, V> w[U];
 #pragma unroll
-    for (int i = 0; i < W; ++i) lds[i * kGnThreads + threadIdx.x] = a[i];
-    for (int have = l.ty; have > 1;) {
-        const int half = (have + 1) >> 1;
-        __syncthreads();
-        if (l.live && l.row + half < have) {
+        for (int u = 0; u < U; ++u)
+            if (r + u * l.ty < r1) w[u] = gn_read<T, V>(x + (r + u * l.ty) * c + l.col);
 #pragma unroll
-            for (int i = 0; i < W; ++i) lds[i * kGnThreads + threadIdx.x] += lds[i * kGnThreads + threadIdx.x + half * l.tx];
-        }
-        have = half;
+        for (int u = 0; u < U; ++u)
+            if (r + u * l.ty < r1) f(w[u], r + u * l.ty);
     }
-    __syncthreads();
 }
 
+// partial [n][groups][chunks]: (sum, sum of squares)
 template <typename T, int V>
 __global__ __launch_bounds__(kGnThreads) void gn_sums_kernel(const T* __restrict__ x, GnShape s, double2* __restrict__ partial) {
-    __shared__ double lds[2 * V * kGnThreads];
-    __shared__ double2 group[kGnMaxGroups];
+    __shared__ double lds[2 * kGnThreads], res[2 * kGnThreads];
+    double2* group = reinterpret_cast<double2*>(gn_lds);
     const int n = blockIdx.x / s.chunks, chunk = blockIdx.x - n * s.chunks;
     const int64_t r0 = chunk * s.chunk_rows, r1 = r0 + s.chunk_rows < s.rows ? r0 + s.chunk_rows : s.rows;
     x += (int64_t)n * s.rows * s.c;
@@ -128,72 +456,54 @@ __global__ __launch_bounds__(kGnThreads) void gn_sums_kernel(const T* __restrict
     const int tiles = (s.c + kGnThreads * V - 1) / (kGnThreads * V);
     for (int tile = 0; tile < tiles; ++tile) {
         const GnLanes l = gn_lanes<V>(s.c, tile);
-        double a[2 * V];
+        double a[2] = {0.0, 0.0};
+        if (l.live)
+            gn_rows<T, V, gn_unroll<T, V>()>(x, s.c, l, r0, r1, [&](const GnPack<T, V>& w, int64_t) {
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) a[i] = 0.0;
-        if (l.live) {
-            for (int64_t r = r0 + l.row; r < r1; r += kGnUnroll * l.ty) {
-                GnPack<T, V> w[kGnUnroll];
-#pragma unroll
-                for (int u = 0; u < kGnUnroll; ++u)
-                    if (r + u * l.ty < r1) w[u] = gn_read<T, V>(x + (r + u * l.ty) * s.c + l.col);
-#pragma unroll
-                for (int u = 0; u < kGnUnroll; ++u)
-                    if (r + u * l.ty < r1) {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            const double v = (double)gn_float(w[u].v[i]);
-                            a[i] += v;
-                            a[V + i] = fma(v, v, a[V + i]);
-                        }
-                    }
-            }
-        }
-        gn_sum_rows<double, 2 * V>(a, l, lds);
-        // channels -> groups: a wave per group that begins in or reaches into this tile
-        const int c0 = tile * kGnThreads * V, c1 = c0 + l.tx * V;
-        for (int g = c0 / s.cg + (int)(threadIdx.x >> 6); g * s.cg < c1 && g < s.groups; g += kGnThreads / kWave) {
-            const int b = g * s.cg > c0 ? g * s.cg : c0, e = (g + 1) * s.cg < c1 ? (g + 1) * s.cg : c1;
+                for (int i = 0; i < V; ++i) {
+                    const double d = (double)gn_float(w.v[i]);
+                    a[0] += d;
+                    a[1] = fma(d, d, a[1]);
+                }
+            });
+        gn_sum_rows<double, 2>(a, l.tx, l.ty, l.row, res, lds);
+        // columns -> the groups that begin in or reach into this tile
+        const int per = s.cg / V, k0 = tile * kGnThreads, k1 = k0 + l.tx, g0 = k0 / per;
+        gn_each_group((k1 - 1) / per - g0 + 1, per, [&](int j, int lane, int lanes) {
+            const int g = g0 + j, b = g * per > k0 ? g * per : k0, e = (g + 1) * per < k1 ? (g + 1) * per : k1;
             double sum = 0.0, sq = 0.0;
-            for (int ch = b + lane_id(); ch < e; ch += kWave) {
-                const int v = (ch - c0) / V, i = (ch - c0) - v * V;
-                sum += lds[i * kGnThreads + v];
-                sq += lds[(V + i) * kGnThreads + v];
+            for (int k = b + lane; k < e; k += lanes) {
+                sum += res[k - k0];
+                sq += res[l.tx + k - k0];
             }
-            sum = wave_sum(sum);
-            sq = wave_sum(sq);
-            if (lane_id() == 0) group[g] = make_double2(group[g].x + sum, group[g].y + sq);
-        }
+            sum = gn_lanes_sum(sum, lanes);
+            sq = gn_lanes_sum(sq, lanes);
+            if (lane == 0) group[g] = make_double2(group[g].x + sum, group[g].y + sq);
+        });
+        __syncthreads();
     }
-    __syncthreads();
-    for (int g = threadIdx.x; g < s.groups; g += kGnThreads) partial[((int64_t)n * s.chunks + chunk) * s.groups + g] = group[g];
+    for (int g = threadIdx.x; g < s.groups; g += kGnThreads) partial[((int64_t)n * s.groups + g) * s.chunks + chunk] = group[g];
 }
 
 // a wave per (sample, group): mean and 1 / sqrt(var + eps)
 __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const double2* __restrict__ partial, GnShape s, double eps, double2* __restrict__ stats) {
     const int64_t at = (int64_t)blockIdx.x * (kGnThreads / kWave) + (threadIdx.x >> 6);
     if (at >= (int64_t)s.n * s.groups) return;
-    const int64_t n = at / s.groups, g = at - n * s.groups;
     double sum = 0.0, sq = 0.0;
+#pragma unroll 4
     for (int k = lane_id(); k < s.chunks; k += kWave) {
-        const double2 p = partial[(n * s.chunks + k) * s.groups + g];
+        const double2 p = partial[at * s.chunks + k];
         sum += p.x;
         sq += p.y;
     }
     sum = wave_sum(sum);
     sq = wave_sum(sq);
-    if (lane_id() == 0) {
-        const double m = (double)s.rows * s.cg, mean = sum / m;
-        double var = sq / m - mean * mean;
-        var = var < 0.0 ? 0.0 : var;                                   // (NaN stays)
-        stats[at] = make_double2(mean, 1.0 / sqrt(var + eps));
-    }
+    if (lane_id() == 0) stats[at] = gn_statistics(sum, sq, (double)s.rows * s.cg, eps);
 }
 
-// ------------------------------------------------------------------------------------------------ y
-template <typename T, int V, int ACT>
-__global__ __launch_bounds__(kGnThreads) void gn_forward_kernel(const T* __restrict__ x, GnShape s, const double2* __restrict__ stats,
-                                                               const void* gamma, const void* beta, int wdtype, T* __restrict__ y) {
+template <typename T, int V>
+__global__ __launch_bounds__(kGnThreads) void gn_forward_kernel(const T* __restrict__ x, GnShape s, const double2* __restrict__ stats, GnWeights w,
+                                                               int act, T* __restrict__ y) {
     const int n = blockIdx.x / s.chunks, chunk = blockIdx.x - n * s.chunks;
     const int64_t r0 = chunk * s.chunk_rows, r1 = r0 + s.chunk_rows < s.rows ? r0 + s.chunk_rows : s.rows;
     const int64_t base = (int64_t)n * s.rows * s.c;
@@ -201,120 +511,94 @@ __global__ __launch_bounds__(kGnThreads) void gn_forward_kernel(const T* __restr
     for (int tile = 0; tile < tiles; ++tile) {
         const GnLanes l = gn_lanes<V>(s.c, tile);
         if (!l.live) continue;
-        float mh[V], ml[V], sc[V], sh[V];
+        GnScale<V> ch;
+        ch.load(stats[(int64_t)n * s.groups + l.col / s.cg], w, l.col);
+        gn_by_act(act, [&](auto A) {
+            gn_rows<T, V, gn_unroll<T, V>()>(x + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, int64_t r) {
+                float o[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const double2 st = stats[(int64_t)n * s.groups + (l.col + i) / s.cg];
-            mh[i] = (float)st.x;
-            ml[i] = (float)(st.x - (double)mh[i]);
-            sc[i] = (float)(st.y * (double)gn_weight(gamma, wdtype, l.col + i, 1.f));
-            sh[i] = gn_weight(beta, wdtype, l.col + i, 0.f);
-        }
-        for (int64_t r = r0 + l.row; r < r1; r += kGnUnroll * l.ty) {
-            GnPack<T, V> w[kGnUnroll];
-#pragma unroll
-            for (int u = 0; u < kGnUnroll; ++u)
-                if (r + u * l.ty < r1) w[u] = gn_read<T, V>(x + base + (r + u * l.ty) * s.c + l.col);
-#pragma unroll
-            for (int u = 0; u < kGnUnroll; ++u)
-                if (r + u * l.ty < r1) {
-                    GnPack<T, V> o;
-#pragma unroll
-                    for (int i = 0; i < V; ++i) o.v[i] = gn_narrow<T>(gn_act<ACT>(((gn_float(w[u].v[i]) - mh[i]) - ml[i]) * sc[i] + sh[i]));
-                    *reinterpret_cast<GnPack<T, V>*>(y + base + (r + u * l.ty) * s.c + l.col) = o;
-                }
-        }
+                for (int i = 0; i < V; ++i) o[i] = ch.template value<decltype(A)::value>(i, gn_float(v.v[i]));
+                gn_write<T, V>(y + base + r * s.c + l.col, o);
+            });
+        });
     }
 }
 
-// ------------------------------------------------------------------------------------------------ gradients
-// what a lane keeps of its V channels for xhat and dz
-template <int V, int ACT> struct GnChannels {
-    float mh[V], ml[V], rstd[V], gamma[V], beta[V], sign[V], thr[V];
-    __device__ __forceinline__ void load(const GnShape& s, const double2* stats, const void* g, const void* b, int wdtype, int n, int col) {
+// two tensors at once, half the rows in flight of each
+template <typename T, int V, int U, typename F>
+__device__ __forceinline__ void gn_rows2(const T* x, const T* dy, int c, const GnLanes& l, int64_t r0, int64_t r1, F f) {
+    for (int64_t r = r0 + l.row; r < r1; r += U * l.ty) {
+        GnPack<T, V> w[U], d[U];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const double2 st = stats[(int64_t)n * s.groups + (col + i) / s.cg];
-            mh[i] = (float)st.x;
-            ml[i] = (float)(st.x - (double)mh[i]);
-            rstd[i] = (float)st.y;
-            gamma[i] = gn_weight(g, wdtype, col + i, 1.f);
-            beta[i] = gn_weight(b, wdtype, col + i, 0.f);
-            if constexpr (ACT == kGnRelu) gn_threshold(st.x, st.y * (double)gamma[i], (double)beta[i], sign[i], thr[i]);
-        }
+        for (int u = 0; u < U; ++u)
+            if (r + u * l.ty < r1) {
+                w[u] = gn_read<T, V>(x + (r + u * l.ty) * c + l.col);
+                d[u] = gn_read<T, V>(dy + (r + u * l.ty) * c + l.col);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r + u * l.ty < r1) f(w[u], d[u], r + u * l.ty);
     }
-    __device__ __forceinline__ void value(int i, float x, float dy, float& xhat, float& dz) const {
-        xhat = ((x - mh[i]) - ml[i]) * rstd[i];
-        if constexpr (ACT == kGnRelu) dz = x * sign[i] > thr[i] ? dy : 0.f;
-        else dz = dy * gn_slope<ACT>(xhat * gamma[i] + beta[i]);
-    }
-};
+}
 
 // per (sample, chunk, channel): (sum dz, sum dz xhat)
-template <typename T, int V, int ACT>
+template <typename T, int V>
 __global__ __launch_bounds__(kGnThreads) void gn_grad_sums_kernel(const T* __restrict__ x, const T* __restrict__ dy, GnShape s,
-                                                                 const double2* __restrict__ stats, const void* gamma, const void* beta,
-                                                                 int wdtype, float2* __restrict__ partial) {
-    __shared__ float lds[2 * V * kGnThreads];
+                                                                 const double2* __restrict__ stats, GnWeights w, int act, float2* __restrict__ partial) {
+    __shared__ float lds[V * kGnThreads], res[2 * V * kGnThreads];
     const int n = blockIdx.x / s.chunks, chunk = blockIdx.x - n * s.chunks;
     const int64_t r0 = chunk * s.chunk_rows, r1 = r0 + s.chunk_rows < s.rows ? r0 + s.chunk_rows : s.rows;
     const int64_t base = (int64_t)n * s.rows * s.c;
     const int tiles = (s.c + kGnThreads * V - 1) / (kGnThreads * V);
     for (int tile = 0; tile < tiles; ++tile) {
         const GnLanes l = gn_lanes<V>(s.c, tile);
-        float a[2 * V];
+        float a[V], b[V];
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) a[i] = 0.f;
+        for (int i = 0; i < V; ++i) a[i] = b[i] = 0.f;
         if (l.live) {
-            GnChannels<V, ACT> ch;
-            ch.load(s, stats, gamma, beta, wdtype, n, l.col);
-            for (int64_t r = r0 + l.row; r < r1; r += kGnUnroll * l.ty) {
-                GnPack<T, V> w[kGnUnroll], d[kGnUnroll];
+            GnGrad<V> ch;
+            ch.load(stats[(int64_t)n * s.groups + l.col / s.cg], w, act, l.col);
+            gn_by_act(act, [&](auto A) {
+                gn_rows2<T, V, (gn_unroll<T, V>() + 1) / 2>(x + base, dy + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, const GnPack<T, V>& d, int64_t) {
 #pragma unroll
-                for (int u = 0; u < kGnUnroll; ++u)
-                    if (r + u * l.ty < r1) {
-                        w[u] = gn_read<T, V>(x + base + (r + u * l.ty) * s.c + l.col);
-                        d[u] = gn_read<T, V>(dy + base + (r + u * l.ty) * s.c + l.col);
+                    for (int i = 0; i < V; ++i) {
+                        float xhat, dz;
+                        ch.template value<decltype(A)::value>(i, gn_float(v.v[i]), gn_float(d.v[i]), xhat, dz);
+                        a[i] += dz;
+                        b[i] = fmaf(dz, xhat, b[i]);
                     }
-#pragma unroll
-                for (int u = 0; u < kGnUnroll; ++u)
-                    if (r + u * l.ty < r1) {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            float xhat, dz;
-                            ch.value(i, gn_float(w[u].v[i]), gn_float(d[u].v[i]), xhat, dz);
-                            a[i] += dz;
-                            a[V + i] += dz * xhat;
-                        }
-                    }
-            }
+                });
+            });
         }
-        gn_sum_rows<float, 2 * V>(a, l, lds);
-        if (l.live && l.row == 0) {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                partial[((int64_t)n * s.chunks + chunk) * s.c + l.col + i] =
-                    make_float2(lds[i * kGnThreads + threadIdx.x], lds[(V + i) * kGnThreads + threadIdx.x]);
+        gn_sum_rows<float, V>(a, l.tx, l.ty, l.row, res, lds);
+        gn_sum_rows<float, V>(b, l.tx, l.ty, l.row, res + V * l.tx, lds);
+        for (int c = threadIdx.x; c < l.tx * V; c += kGnThreads) {
+            const int k = c / V, i = c - k * V;
+            partial[((int64_t)n * s.chunks + chunk) * s.c + tile * kGnThreads * V + c] = make_float2(res[i * l.tx + k], res[(V + i) * l.tx + k]);
         }
+        __syncthreads();
     }
 }
 
 // a workgroup per (sample, group): the channels' sums over the chunks, and the group's two means
-__global__ __launch_bounds__(kGnThreads) void gn_grad_stats_kernel(const float2* __restrict__ partial, GnShape s, const void* gamma, int wdtype,
-                                                                  double2* __restrict__ channel, float2* __restrict__ means) {
-    __shared__ double2 lds[kGnThreads];
+constexpr int kGnStatThreads = 512;
+__global__ __launch_bounds__(kGnStatThreads) void gn_grad_stats_kernel(const float2* __restrict__ partial, GnShape s, GnWeights w,
+                                                                      double2* __restrict__ channel, float2* __restrict__ means) {
+    __shared__ double2 lds[kGnStatThreads];
     const int n = blockIdx.x / s.groups, g = blockIdx.x - n * s.groups;
     double s1 = 0.0, s2 = 0.0;
-    for (int c0 = 0; c0 < s.cg; c0 += kGnThreads) {
-        const int tx = s.cg - c0 < kGnThreads ? s.cg - c0 : kGnThreads, ty = kGnThreads / tx;
+    for (int c0 = 0; c0 < s.cg; c0 += kGnStatThreads) {
+        const int tx = s.cg - c0 < kGnStatThreads ? s.cg - c0 : kGnStatThreads, ty = kGnStatThreads / tx;
         const int row = threadIdx.x / tx, ch = g * s.cg + c0 + (threadIdx.x - row * tx);
         double2 acc = make_double2(0.0, 0.0);
-        if (row < ty)
+        if (row < ty) {
+#pragma unroll 8
             for (int k = row; k < s.chunks; k += ty) {
                 const float2 p = partial[((int64_t)n * s.chunks + k) * s.c + ch];
                 acc.x += p.x;
                 acc.y += p.y;
             }
+        }
         __syncthreads();
         lds[threadIdx.x] = acc;
         for (int have = ty; have > 1;) {
@@ -330,9 +614,9 @@ __global__ __launch_bounds__(kGnThreads) void gn_grad_stats_kernel(const float2*
         if (row == 0) {
             const double2 sum = lds[threadIdx.x];
             channel[(int64_t)n * s.c + ch] = sum;
-            const double w = (double)gn_weight(gamma, wdtype, ch, 1.f);
-            s1 += w * sum.x;
-            s2 += w * sum.y;
+            const double gm = (double)gn_weight(w.gamma, w.dtype, ch, 1.f);
+            s1 += gm * sum.x;
+            s2 += gm * sum.y;
         }
     }
     s1 = wave_sum(s1);
@@ -341,23 +625,17 @@ __global__ __launch_bounds__(kGnThreads) void gn_grad_stats_kernel(const float2*
     if (lane_id() == 0) lds[threadIdx.x >> 6] = make_double2(s1, s2);
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kGnThreads / kWave; ++w) { s1 += lds[w].x; s2 += lds[w].y; }
+        for (int k = 1; k < kGnStatThreads / kWave; ++k) { s1 += lds[k].x; s2 += lds[k].y; }
         const double m = (double)s.rows * s.cg;
         means[(int64_t)n * s.groups + g] = make_float2((float)(s1 / m), (float)(s2 / m));
     }
-}
-
-__device__ __forceinline__ void gn_store_weight(void* w, int dtype, int c, float v) {
-    if (!w) return;
-    if (dtype == GEOMAE_DTYPE_F32) static_cast<float*>(w)[c] = v;
-    else if (dtype == GEOMAE_DTYPE_BF16) static_cast<uint16_t*>(w)[c] = gn_narrow<uint16_t>(v);
-    else static_cast<_Float16*>(w)[c] = gn_narrow<_Float16>(v);
 }
 
 // d gamma, d beta: the samples' sums of a channel, a channel per thread over the launch's first workgroups
 __device__ __forceinline__ void gn_weight_grad(const double2* channel, int rows, int c, int wdtype, void* dgamma, void* dbeta, int block, int blocks) {
     for (int64_t ch = (int64_t)block * kGnThreads + threadIdx.x; ch < c; ch += (int64_t)blocks * kGnThreads) {
         double a = 0.0, b = 0.0;
+#pragma unroll 4
         for (int n = 0; n < rows; ++n) {
             const double2 p = channel[(int64_t)n * c + ch];
             a += p.x;
@@ -384,67 +662,77 @@ __global__ __launch_bounds__(kGnThreads) void gn_fold_kernel(const double2* __re
     out[at] = acc;
 }
 
-template <typename T, int V, int ACT>
+template <typename T, int V>
 __global__ __launch_bounds__(kGnThreads) void gn_backward_kernel(const T* __restrict__ x, const T* __restrict__ dy, GnShape s,
-                                                                const double2* __restrict__ stats, const void* gamma, const void* beta,
-                                                                int wdtype, const double2* __restrict__ channel,
-                                                                const float2* __restrict__ means, T* __restrict__ dx, void* dgamma, void* dbeta) {
+                                                                const double2* __restrict__ stats, GnWeights w, int act,
+                                                                const double2* __restrict__ channel, const float2* __restrict__ means,
+                                                                T* __restrict__ dx, void* dgamma, void* dbeta) {
     const int n = blockIdx.x / s.chunks, chunk = blockIdx.x - n * s.chunks;
     const int64_t r0 = chunk * s.chunk_rows, r1 = r0 + s.chunk_rows < s.rows ? r0 + s.chunk_rows : s.rows;
     const int64_t base = (int64_t)n * s.rows * s.c;
-    if (dgamma || dbeta) gn_weight_grad(channel, s.n, s.c, wdtype, dgamma, dbeta, blockIdx.x, gridDim.x);
+    if (dgamma || dbeta) gn_weight_grad(channel, s.n, s.c, w.dtype, dgamma, dbeta, blockIdx.x, gridDim.x);
     const int tiles = (s.c + kGnThreads * V - 1) / (kGnThreads * V);
     for (int tile = 0; tile < tiles; ++tile) {
         const GnLanes l = gn_lanes<V>(s.c, tile);
         if (!l.live) continue;
-        GnChannels<V, ACT> ch;
-        ch.load(s, stats, gamma, beta, wdtype, n, l.col);
-        float s1[V], s2[V];
+        GnGrad<V> ch;
+        ch.load(stats[(int64_t)n * s.groups + l.col / s.cg], w, act, l.col);
+        const float2 mean = means[(int64_t)n * s.groups + l.col / s.cg];
+        const float c1 = ch.rstd * mean.x, c2 = ch.rstd * mean.y;
+        gn_by_act(act, [&](auto A) {
+            gn_rows2<T, V, (gn_unroll<T, V>() + 1) / 2>(x + base, dy + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, const GnPack<T, V>& d, int64_t r) {
+                float o[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float2 m = means[(int64_t)n * s.groups + (l.col + i) / s.cg];
-            s1[i] = m.x;
-            s2[i] = m.y;
-        }
-        for (int64_t r = r0 + l.row; r < r1; r += kGnUnroll * l.ty) {
-            GnPack<T, V> w[kGnUnroll], d[kGnUnroll];
-#pragma unroll
-            for (int u = 0; u < kGnUnroll; ++u)
-                if (r + u * l.ty < r1) {
-                    w[u] = gn_read<T, V>(x + base + (r + u * l.ty) * s.c + l.col);
-                    d[u] = gn_read<T, V>(dy + base + (r + u * l.ty) * s.c + l.col);
+                for (int i = 0; i < V; ++i) {
+                    float xhat, dz;
+                    ch.template value<decltype(A)::value>(i, gn_float(v.v[i]), gn_float(d.v[i]), xhat, dz);
+                    o[i] = ch.dx(i, xhat, dz, c1, c2);
                 }
-#pragma unroll
-            for (int u = 0; u < kGnUnroll; ++u)
-                if (r + u * l.ty < r1) {
-                    GnPack<T, V> o;
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        float xhat, dz;
-                        ch.value(i, gn_float(w[u].v[i]), gn_float(d[u].v[i]), xhat, dz);
-                        o.v[i] = gn_narrow<T>(ch.rstd[i] * (ch.gamma[i] * dz - s1[i] - xhat * s2[i]));
-                    }
-                    *reinterpret_cast<GnPack<T, V>*>(dx + base + (r + u * l.ty) * s.c + l.col) = o;
-                }
-        }
+                gn_write<T, V>(dx + base + r * s.c + l.col, o);
+            });
+        });
     }
 }
 
 // ------------------------------------------------------------------------------------------------ host
-static int gn_vector(int c, int dtype) {           // channels of a lane: 16 bytes where they divide c, else 4 bytes or one
-    if (dtype == GEOMAE_DTYPE_F32) return c % 4 == 0 ? 4 : 1;
-    return c % 8 == 0 ? 8 : (c % 2 == 0 ? 2 : 1);
+static int gn_vector(int cg, int most) {           // channels of a thread, all of one group
+    for (int v = most; v > 1; v >>= 1)
+        if (cg % v == 0) return v;
+    return 1;
 }
-static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype) {
+static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype, bool backward) {
     GnShape s;
     s.n = n; s.rows = rows; s.c = c; s.groups = groups; s.cg = c / groups;
-    const int cv = c / gn_vector(c, dtype), ty = cv < kGnThreads ? kGnThreads / cv : 1;
-    const int64_t least = (int64_t)ty * kGnUnroll, wanted = kGnBlocks / n > 1 ? kGnBlocks / n : 1;
+    const int item = dtype == GEOMAE_DTYPE_F32 ? 4 : 2;
+    // resident, if all rows of a group fit; more groups to a workgroup while its piece of a row is short of a cache line and there
+    // are workgroups for every CU without
+    s.v = gn_vector(s.cg, 4);
+    s.cs = s.threads = 0;
+    const int held = gn_vectors_held(s.v, item);
+    auto fits = [&](int64_t cs) {
+        const int64_t tx = cs / s.v;
+        return tx <= kGnResidentThreads && rows <= kGnResidentThreads / tx * held;
+    };
+    if (fits(s.cg)) {
+        int k = 1;
+        for (int d = 2; d <= groups && (int64_t)k * s.cg * item < 128; ++d)
+            if (groups % d == 0 && fits((int64_t)d * s.cg) && (int64_t)n * (groups / d) >= 256) k = d;
+        s.cs = k * s.cg;
+        const int64_t tx = s.cs / s.v;
+        // (two vectors a thread: enough loads in flight, and half the threads to add up)
+        int64_t threads = (tx * ((rows + 1) / 2) + kWave - 1) / kWave * kWave;
+        threads = threads > kGnResidentThreads ? kGnResidentThreads : threads;
+        while (threads < tx || threads / tx * held < rows) threads += kWave;
+        s.threads = (int32_t)threads;
+    } else if (!backward && item == 2) s.v = gn_vector(s.cg, 8);
+    const int cv = c / s.v, ty = cv < kGnThreads ? kGnThreads / cv : 1, unroll = 64 / (s.v * item) < 16 ? 64 / (s.v * item) : 16;
+    const int64_t least = (int64_t)ty * unroll, wanted = kGnBlocks / n > 1 ? kGnBlocks / n : 1;
     s.chunk_rows = (rows + wanted - 1) / wanted;
     s.chunk_rows = s.chunk_rows < least ? least : (s.chunk_rows + least - 1) / least * least;
-    s.chunks = (int32_t)((rows + s.chunk_rows - 1) / s.chunk_rows);
+    s.chunks = s.cs ? 0 : (int32_t)((rows + s.chunk_rows - 1) / s.chunk_rows);
     return s;
 }
+static int64_t gn_pad(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 struct GnWorkspace { double2* partial; float2* grad_partial; double2 *channel, *folded; float2* means; int64_t forward_bytes, backward_bytes; };
 static GnWorkspace gn_workspace(void* base, const GnShape& s) {
     char* p = static_cast<char*>(base);
@@ -452,74 +740,58 @@ static GnWorkspace gn_workspace(void* base, const GnShape& s) {
     w.partial = reinterpret_cast<double2*>(p);
     w.forward_bytes = (int64_t)s.n * s.chunks * s.groups * (int64_t)sizeof(double2);
     w.channel = reinterpret_cast<double2*>(p);
-    const int64_t a = (int64_t)s.n * s.c * (int64_t)sizeof(double2);
-    w.grad_partial = reinterpret_cast<float2*>(p + a);
-    const int64_t b = a + ((int64_t)s.n * s.chunks * s.c * (int64_t)sizeof(float2) + 15) / 16 * 16;
-    w.means = reinterpret_cast<float2*>(p + b);
-    const int64_t d = b + ((int64_t)s.n * s.groups * (int64_t)sizeof(float2) + 15) / 16 * 16;
-    w.folded = reinterpret_cast<double2*>(p + d);                      // two halves, used in turn
-    w.backward_bytes = d + (s.n > kGnFold ? 2 * (int64_t)((s.n + kGnFold - 1) / kGnFold) * s.c * (int64_t)sizeof(double2) : 0);
+    int64_t at = s.cs && s.n == 1 ? 0 : (int64_t)s.n * s.c * (int64_t)sizeof(double2);
+    w.grad_partial = reinterpret_cast<float2*>(p + at);
+    at += gn_pad((int64_t)s.n * s.chunks * s.c * (int64_t)sizeof(float2));
+    w.means = reinterpret_cast<float2*>(p + at);
+    at += s.cs ? 0 : gn_pad((int64_t)s.n * s.groups * (int64_t)sizeof(float2));
+    w.folded = reinterpret_cast<double2*>(p + at);                     // two halves, used in turn
+    w.backward_bytes = at + (s.n > kGnFold ? 2 * (int64_t)((s.n + kGnFold - 1) / kGnFold) * s.c * (int64_t)sizeof(double2) : 0);
     return w;
+}
+// dynamic LDS of the resident kernels: the groups' values, the columns' sums, and what gn_sum_rows works in
+static size_t gn_resident_lds(const GnShape& s, bool backward) {
+    const int v = s.v;
+    const int64_t tx = s.cs / v, item = backward ? 4 : 8, width = backward ? v : 2;
+    const int64_t rows = tx <= kWave / 2 && (tx & (tx - 1)) == 0 ? (int64_t)s.threads / kWave * tx : s.threads;
+    return (size_t)(s.cs / s.cg * (backward ? 8 : 16) + ((backward ? 2 * v : 2) * tx + width * rows) * item);
 }
 static int gn_check(const char* what, int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype, int wdtype, int act) {
     GEOMAE_REQUIRE(n >= 0 && rows >= 0 && c > 0 && groups > 0, "%s: bad shape [%d, %lld, %d] in %d groups", what, (int)n,
                    (long long)rows, (int)c, (int)groups);
     GEOMAE_REQUIRE(c % groups == 0, "%s: %d channels do not divide into %d groups", what, (int)c, (int)groups);
     GEOMAE_REQUIRE(groups <= kGnMaxGroups, "%s: at most %d groups, got %d", what, kGnMaxGroups, (int)groups);
-    GEOMAE_REQUIRE((int64_t)n * groups <= INT32_MAX && c <= INT32_MAX / 16, "%s: %d samples of %d groups are too many", what, (int)n, (int)groups);
+    GEOMAE_REQUIRE((int64_t)n * groups <= INT32_MAX && (int64_t)n * kGnBlocks <= INT32_MAX && c <= INT32_MAX / 16, "%s: %d samples of %d groups are too many", what,
+                   (int)n, (int)groups);
     GEOMAE_REQUIRE(dtype >= 0 && dtype <= 2 && wdtype >= 0 && wdtype <= 2, "%s: unknown dtype", what);
     GEOMAE_REQUIRE(act >= 0 && act <= 3, "%s: unknown activation %d", what, act);
     return GEOMAE_OK;
 }
-
-template <typename T, int V, int ACT>
-static void gn_launch_forward(const void* x, const GnShape& s, const double2* stats, const void* gamma, const void* beta, int wdtype, void* y, hipStream_t stream) {
-    hipLaunchKernelGGL((gn_forward_kernel<T, V, ACT>), dim3(s.chunks * s.n), dim3(kGnThreads), 0, stream, static_cast<const T*>(x), s, stats, gamma, beta,
-                       wdtype, static_cast<T*>(y));
-}
-struct GnBackward { const void *x, *dy, *gamma, *beta; const double2* stats; void *dx, *dgamma, *dbeta; int wdtype; };
-template <typename T, int V, int ACT>
-static void gn_launch_backward(const GnBackward& b, const GnShape& s, const GnWorkspace& w, hipStream_t stream) {
-    hipLaunchKernelGGL((gn_grad_sums_kernel<T, V, ACT>), dim3(s.chunks * s.n), dim3(kGnThreads), 0, stream, static_cast<const T*>(b.x),
-                       static_cast<const T*>(b.dy), s, b.stats, b.gamma, b.beta, b.wdtype, w.grad_partial);
-    hipLaunchKernelGGL(gn_grad_stats_kernel, dim3(s.groups * s.n), dim3(kGnThreads), 0, stream, w.grad_partial, s, b.gamma, b.wdtype, w.channel, w.means);
-    const bool many = s.n > kGnFold;
-    hipLaunchKernelGGL((gn_backward_kernel<T, V, ACT>), dim3(s.chunks * s.n), dim3(kGnThreads), 0, stream, static_cast<const T*>(b.x),
-                       static_cast<const T*>(b.dy), s, b.stats, b.gamma, b.beta, b.wdtype, w.channel, w.means, static_cast<T*>(b.dx),
-                       many ? nullptr : b.dgamma, many ? nullptr : b.dbeta);
-    if (!many || !(b.dgamma || b.dbeta)) return;
-    const double2* from = w.channel;
+static void gn_launch_weight_grad(const double2* channel, int rows, const GnShape& s, const GnWorkspace& w, int wdtype, void* dgamma, void* dbeta, hipStream_t stream) {
     double2* halves[2] = {w.folded, w.folded + (int64_t)((s.n + kGnFold - 1) / kGnFold) * s.c};
-    int rows = s.n;
     for (int k = 0; rows > kGnFold; ++k) {
         const int next = (rows + kGnFold - 1) / kGnFold;
-        hipLaunchKernelGGL(gn_fold_kernel, dim3(cdiv((int64_t)next * s.c, kGnThreads)), dim3(kGnThreads), 0, stream, from, rows, s.c, halves[k & 1]);
-        from = halves[k & 1];
+        hipLaunchKernelGGL(gn_fold_kernel, dim3(cdiv((int64_t)next * s.c, kGnThreads)), dim3(kGnThreads), 0, stream, channel, rows, s.c, halves[k & 1]);
+        channel = halves[k & 1];
         rows = next;
     }
-    hipLaunchKernelGGL(gn_weight_grad_kernel, dim3(cdiv(s.c, kGnThreads)), dim3(kGnThreads), 0, stream, from, rows, s.c, b.wdtype, b.dgamma, b.dbeta);
+    hipLaunchKernelGGL(gn_weight_grad_kernel, dim3(cdiv(s.c, kGnThreads)), dim3(kGnThreads), 0, stream, channel, rows, s.c, wdtype, dgamma, dbeta);
 }
-// f(type, vector, activation) for the run-time choice of the three
-template <typename F> static void gn_by_act(int act, F f) {
-    if (act == kGnRelu) f(std::integral_constant<int, kGnRelu>());
-    else if (act == kGnSilu) f(std::integral_constant<int, kGnSilu>());
-    else if (act == kGnGelu) f(std::integral_constant<int, kGnGelu>());
-    else f(std::integral_constant<int, kGnNone>());
-}
+
+// f(type, vector) for the run-time choice of the two
 template <typename T> struct GnType { typedef T type; };
-template <typename F> static void gn_by_type(int dtype, int v, F f) {
-    if (dtype == GEOMAE_DTYPE_F32) {
-        if (v == 4) f(GnType<float>(), std::integral_constant<int, 4>());
-        else f(GnType<float>(), std::integral_constant<int, 1>());
-    } else if (dtype == GEOMAE_DTYPE_BF16) {
-        if (v == 8) f(GnType<uint16_t>(), std::integral_constant<int, 8>());
-        else if (v == 2) f(GnType<uint16_t>(), std::integral_constant<int, 2>());
-        else f(GnType<uint16_t>(), std::integral_constant<int, 1>());
-    } else {
-        if (v == 8) f(GnType<_Float16>(), std::integral_constant<int, 8>());
-        else if (v == 2) f(GnType<_Float16>(), std::integral_constant<int, 2>());
-        else f(GnType<_Float16>(), std::integral_constant<int, 1>());
+template <typename T, int MOST, typename F> static void gn_by_vector(int v, F f) {
+    if constexpr (MOST == 8) {
+        if (v == 8) return f(GnType<T>(), std::integral_constant<int, 8>());
     }
+    if (v == 4) f(GnType<T>(), std::integral_constant<int, 4>());
+    else if (v == 2) f(GnType<T>(), std::integral_constant<int, 2>());
+    else f(GnType<T>(), std::integral_constant<int, 1>());
+}
+template <int MOST16, typename F> static void gn_by_type(int dtype, int v, F f) {
+    if (dtype == GEOMAE_DTYPE_F32) gn_by_vector<float, 4>(v, f);
+    else if (dtype == GEOMAE_DTYPE_BF16) gn_by_vector<uint16_t, MOST16>(v, f);
+    else gn_by_vector<_Float16, MOST16>(v, f);
 }
 
 }  // namespace geomae
@@ -529,7 +801,7 @@ using namespace geomae;
 extern "C" int64_t geomae_group_norm_workspace_bytes(int32_t n, int64_t rows, int32_t c, int32_t groups, int32_t dtype, int32_t backward) {
     if (gn_check("group_norm_workspace_bytes", n, rows, c, groups, dtype, 0, 0)) return -1;
     if (n == 0 || rows == 0) return 0;
-    const GnWorkspace w = gn_workspace(nullptr, gn_shape(n, rows, c, groups, dtype));
+    const GnWorkspace w = gn_workspace(nullptr, gn_shape(n, rows, c, groups, dtype, backward != 0));
     return backward ? w.backward_bytes : w.forward_bytes;
 }
 
@@ -540,19 +812,29 @@ extern "C" int geomae_group_norm_forward(const void* x, int32_t dtype, int32_t n
     GEOMAE_REQUIRE(eps >= 0.0, "group_norm_forward: eps must not be negative");
     if (n == 0 || rows == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(x && y && stats, "group_norm_forward: null argument");
-    const GnShape s = gn_shape(n, rows, c, groups, dtype);
-    const GnWorkspace w = gn_workspace(workspace, s);
-    if (!workspace || workspace_bytes < w.forward_bytes) {
-        set_error("group_norm_forward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)w.forward_bytes);
+    const GnShape s = gn_shape(n, rows, c, groups, dtype, false);
+    const GnWorkspace ws = gn_workspace(workspace, s);
+    if (workspace_bytes < ws.forward_bytes || (ws.forward_bytes && !workspace)) {
+        set_error("group_norm_forward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws.forward_bytes);
         return GEOMAE_ERR_WORKSPACE;
     }
     double2* st = reinterpret_cast<double2*>(stats);
-    gn_by_type(dtype, gn_vector(c, dtype), [&](auto t, auto v) {
+    const GnWeights w = {gamma, beta, weight_dtype};
+    if (s.cs) {
+        gn_by_type<4>(dtype, s.v, [&](auto t, auto vec) {
+            typedef typename decltype(t)::type T;
+            hipLaunchKernelGGL((gn_resident_forward_kernel<T, decltype(vec)::value>), dim3(n * (c / s.cs)), dim3(s.threads), gn_resident_lds(s, false), stream,
+                               static_cast<const T*>(x), s, w, eps, activation, static_cast<T*>(y), st);
+        });
+        return check_launch("gn_resident_forward_kernel");
+    }
+    gn_by_type<8>(dtype, s.v, [&](auto t, auto vec) {
         typedef typename decltype(t)::type T;
-        constexpr int V = decltype(v)::value;
-        hipLaunchKernelGGL((gn_sums_kernel<T, V>), dim3(s.chunks * n), dim3(kGnThreads), 0, stream, static_cast<const T*>(x), s, w.partial);
-        hipLaunchKernelGGL(gn_stats_kernel, dim3(cdiv((int64_t)n * groups, kGnThreads / kWave)), dim3(kGnThreads), 0, stream, w.partial, s, eps, st);
-        gn_by_act(activation, [&](auto a) { gn_launch_forward<T, V, decltype(a)::value>(x, s, st, gamma, beta, weight_dtype, y, stream); });
+        constexpr int V = decltype(vec)::value;
+        const T* in = static_cast<const T*>(x);
+        hipLaunchKernelGGL((gn_sums_kernel<T, V>), dim3(s.chunks * n), dim3(kGnThreads), groups * sizeof(double2), stream, in, s, ws.partial);
+        hipLaunchKernelGGL(gn_stats_kernel, dim3(cdiv((int64_t)n * groups, kGnThreads / kWave)), dim3(kGnThreads), 0, stream, ws.partial, s, eps, st);
+        hipLaunchKernelGGL((gn_forward_kernel<T, V>), dim3(s.chunks * n), dim3(kGnThreads), 0, stream, in, s, st, w, activation, static_cast<T*>(y));
     });
     return check_launch("gn_forward_kernel");
 }
@@ -563,17 +845,30 @@ extern "C" int geomae_group_norm_backward(const void* x, const void* dy, int32_t
     if (int rc = gn_check("group_norm_backward", n, rows, c, groups, dtype, weight_dtype, activation)) return rc;
     if (n == 0 || rows == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(x && dy && stats && dx, "group_norm_backward: null argument");
-    const GnShape s = gn_shape(n, rows, c, groups, dtype);
-    const GnWorkspace w = gn_workspace(workspace, s);
-    if (!workspace || workspace_bytes < w.backward_bytes) {
-        set_error("group_norm_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)w.backward_bytes);
+    const GnShape s = gn_shape(n, rows, c, groups, dtype, true);
+    const GnWorkspace ws = gn_workspace(workspace, s);
+    if (workspace_bytes < ws.backward_bytes || (ws.backward_bytes && !workspace)) {
+        set_error("group_norm_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws.backward_bytes);
         return GEOMAE_ERR_WORKSPACE;
     }
-    const GnBackward b = {x, dy, gamma, beta, reinterpret_cast<const double2*>(stats), dx, dgamma, dbeta, weight_dtype};
-    gn_by_type(dtype, gn_vector(c, dtype), [&](auto t, auto v) {
+    const double2* st = reinterpret_cast<const double2*>(stats);
+    const GnWeights w = {gamma, beta, weight_dtype};
+    const bool weights = dgamma || dbeta, many = n > kGnFold;
+    gn_by_type<4>(dtype, s.v, [&](auto t, auto vec) {
         typedef typename decltype(t)::type T;
-        constexpr int V = decltype(v)::value;
-        gn_by_act(activation, [&](auto a) { gn_launch_backward<T, V, decltype(a)::value>(b, s, w, stream); });
+        constexpr int V = decltype(vec)::value;
+        const T *in = static_cast<const T*>(x), *grad = static_cast<const T*>(dy);
+        if (s.cs) {
+            hipLaunchKernelGGL((gn_resident_backward_kernel<T, V>), dim3(n * (c / s.cs)), dim3(s.threads), gn_resident_lds(s, true), stream, in, grad, s,
+                               st, w, activation, static_cast<T*>(dx), n == 1 ? nullptr : ws.channel, dgamma, dbeta);
+            if (weights && n > 1) gn_launch_weight_grad(ws.channel, n, s, ws, weight_dtype, dgamma, dbeta, stream);
+            return;
+        }
+        hipLaunchKernelGGL((gn_grad_sums_kernel<T, V>), dim3(s.chunks * n), dim3(kGnThreads), 0, stream, in, grad, s, st, w, activation, ws.grad_partial);
+        hipLaunchKernelGGL(gn_grad_stats_kernel, dim3(groups * n), dim3(kGnStatThreads), 0, stream, ws.grad_partial, s, w, ws.channel, ws.means);
+        hipLaunchKernelGGL((gn_backward_kernel<T, V>), dim3(s.chunks * n), dim3(kGnThreads), 0, stream, in, grad, s, st, w, activation, ws.channel,
+                           ws.means, static_cast<T*>(dx), many ? nullptr : dgamma, many ? nullptr : dbeta);
+        if (weights && many) gn_launch_weight_grad(ws.channel, n, s, ws, weight_dtype, dgamma, dbeta, stream);
     });
     return check_launch("gn_backward_kernel");
 }

@@ -95,7 +95,8 @@ def make(dev, shape, dtype, seed=0, offset=1.0):
 def check(got, want, label=""):
     value, bound = want
     err = (got.detach().double().reshape(value.shape) - value).abs()
-    assert got.isfinite().all() and (err <= bound).all(), (label, float((err / bound.clamp(min=1e-300)).max()))
+    fine, worst = bool(got.isfinite().all()), float((err / bound.clamp(min=1e-300)).max())
+    assert fine and worst <= 1.0, (label, worst)
 
 
 def run_both(x, groups, w, b, act, dy, eps=1e-5):

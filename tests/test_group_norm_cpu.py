@@ -59,13 +59,14 @@ def test_refusals_need_no_gpu():
 def test_entry_points_check_their_arguments():
     from geomae_amd import _lib
     lib = _lib.load()
-    wsb = lib.geomae_group_norm_workspace_bytes
-    assert wsb(0, 10, 8, 2, 0, 0) == 0 and wsb(2, 0, 8, 2, 0, 1) == 0
-    assert 0 < wsb(2, 10, 8, 2, 0, 0) and 0 < wsb(2, 10, 8, 2, 0, 1) < wsb(200, 10, 8, 2, 0, 1)
-    for bad in ((2, 10, 8, 3, 0, 0), (-1, 10, 8, 2, 0, 0), (2, 10, 0, 1, 0, 0), (2, 10, 8, 2, 3, 0), (2, 10, 4096, 2048, 0, 0)):
+    wsb, rows = lib.geomae_group_norm_workspace_bytes, 100_000            # rows of a group that no workgroup holds
+    assert wsb(0, rows, 8, 2, 0, 0) == 0 and wsb(2, 0, 8, 2, 0, 1) == 0
+    assert 0 < wsb(2, rows, 8, 2, 0, 0) and 0 < wsb(2, rows, 8, 2, 0, 1) < wsb(200, rows, 8, 2, 0, 1)
+    assert wsb(2, 10, 8, 2, 0, 0) >= 0 and wsb(2, 10, 8, 2, 0, 1) > 0
+    for bad in ((2, rows, 8, 3, 0, 0), (-1, rows, 8, 2, 0, 0), (2, rows, 0, 1, 0, 0), (2, rows, 8, 2, 3, 0), (2, rows, 4096, 2048, 0, 0)):
         assert wsb(*bad) == -1, bad
 
-    def forward(x=64, dtype=0, n=2, rows=10, c=8, groups=2, eps=1e-5, act=0, ws=64, bytes_=1 << 20):
+    def forward(x=64, dtype=0, n=2, rows=rows, c=8, groups=2, eps=1e-5, act=0, ws=64, bytes_=1 << 20):
         return lib.geomae_group_norm_forward(x, dtype, n, rows, c, groups, None, None, 0, eps, act, 64, 64, ws, bytes_, None)
     assert forward(n=0) == 0 and forward(rows=0) == 0
     assert forward(x=None) < 0 and b"null" in lib.geomae_last_error()
@@ -74,5 +75,5 @@ def test_entry_points_check_their_arguments():
     assert forward(bytes_=8) == -3 and forward(ws=None) == -3
 
     def backward(dy=64, n=2, bytes_=1 << 20):
-        return lib.geomae_group_norm_backward(64, dy, 0, n, 10, 8, 2, None, None, 0, 0, 64, 64, None, None, 64, bytes_, None)
+        return lib.geomae_group_norm_backward(64, dy, 0, n, rows, 8, 2, None, None, 0, 0, 64, 64, None, None, 64, bytes_, None)
     assert backward(n=0) == 0 and backward(dy=None) < 0 and backward(bytes_=8) == -3
