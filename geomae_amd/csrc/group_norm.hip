@@ -37,8 +37,11 @@ struct GnShape {
     int32_t n, c, groups, cg;
     int32_t chunks;                                // of a sample's rows (streamed)
     int64_t chunk_rows;
+    double inv_m;                                  // 1 / (elements of a group of a sample)
     int32_t v;                                     // channels of a thread
-    int32_t cs, threads;                           // channels of a resident workgroup, 0: streamed; its threads
+    int32_t cs, threads;                           // channels of a resident workgroup, 0: streamed; its threads ...
+    int32_t tx, ty, slabs, slab_groups;            // ... as tx columns x ty rows; workgroups of a sample, groups of a workgroup
+    uint32_t tx_inverse;                           // t / tx = (t * this) >> 20 for t < 1024
 };
 
 template <typename T> __device__ __forceinline__ float gn_float(T x) { return (float)x; }
@@ -143,15 +146,21 @@ struct GnWeights { const void *gamma, *beta; int dtype; };
 // what a lane keeps of its V channels, all of one group, for y
 template <int V> struct GnScale {
     float mean, scale[V], rest[V], beta[V];
-    __device__ __forceinline__ void load(double2 stat, const GnWeights& w, int col) {
+    __device__ __forceinline__ void weights(const GnWeights& w, int col) {          // (scale holds gamma until statistics() is called)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            scale[i] = gn_weight(w.gamma, w.dtype, col + i, 1.f);
+            beta[i] = gn_weight(w.beta, w.dtype, col + i, 0.f);
+        }
+    }
+    __device__ __forceinline__ void statistics(double2 stat) {
         mean = (float)stat.x;
         const double lost = stat.x - (double)mean;                     // what mean's rounding lost comes back behind the product
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const double sc = stat.y * (double)gn_weight(w.gamma, w.dtype, col + i, 1.f);
+            const double sc = stat.y * (double)scale[i];
             scale[i] = (float)sc;
             rest[i] = (float)(-lost * sc);
-            beta[i] = gn_weight(w.beta, w.dtype, col + i, 0.f);
         }
     }
     template <int ACT> __device__ __forceinline__ float value(int i, float x) const { return gn_act<ACT>(fmaf(x - mean, scale[i], rest[i]) + beta[i]); }
@@ -182,17 +191,47 @@ template <int V> struct GnGrad {
 };
 
 // ------------------------------------------------------------------------------------------------ sums over a workgroup
+// v summed over the lanes of a wave that are equal modulo tx (a power of two up to 32), in every lane: the halves and rows by
+// the swaps, within a row of 16 by rotations (by 8, 4, ...: what is equal modulo 8, 4, ... already makes them exchanges)
+template <int CTRL> __device__ __forceinline__ double gn_dpp(double v) {
+    return __hiloint2double(dpp_mov<CTRL>(__double2hiint(v)), dpp_mov<CTRL>(__double2loint(v)));
+}
+template <int CTRL> __device__ __forceinline__ float gn_dpp(float v) { return dpp_mov<CTRL>(v); }
+__device__ __forceinline__ float gn_swap32(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ float gn_swap16(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ double gn_swap32(double v) {
+    const auto h = __builtin_amdgcn_permlane32_swap((uint32_t)__double2hiint(v), (uint32_t)__double2hiint(v), false, false);
+    const auto l = __builtin_amdgcn_permlane32_swap((uint32_t)__double2loint(v), (uint32_t)__double2loint(v), false, false);
+    return __hiloint2double((int)h[0], (int)l[0]) + __hiloint2double((int)h[1], (int)l[1]);
+}
+__device__ __forceinline__ double gn_swap16(double v) {
+    const auto h = __builtin_amdgcn_permlane16_swap((uint32_t)__double2hiint(v), (uint32_t)__double2hiint(v), false, false);
+    const auto l = __builtin_amdgcn_permlane16_swap((uint32_t)__double2loint(v), (uint32_t)__double2loint(v), false, false);
+    return __hiloint2double((int)h[0], (int)l[0]) + __hiloint2double((int)h[1], (int)l[1]);
+}
+template <typename S> __device__ __forceinline__ S gn_wave_columns(S v, int tx) {
+    v = gn_swap32(v);
+    if (tx <= 16) v = gn_swap16(v);
+    if (tx <= 8) v += gn_dpp<0x128>(v);            // row_ror:8
+    if (tx <= 4) v += gn_dpp<0x124>(v);
+    if (tx <= 2) v += gn_dpp<0x122>(v);
+    if (tx <= 1) v += gn_dpp<0x121>(v);
+    return v;
+}
 // a[W] of every thread (row, col) of tx columns x ty rows, summed over the rows: res[w * tx + col].  Fixed order.
-__device__ __forceinline__ bool gn_in_waves(int tx) { return tx <= kWave / 2 && (tx & (tx - 1)) == 0; }
 template <typename S, int W>
 __device__ __forceinline__ void gn_sum_rows(S (&a)[W], int tx, int ty, int row, S* res, S* lds) {
     const int threads = blockDim.x, t = threadIdx.x;
-    if (gn_in_waves(tx)) {                                             // a wave holds whole rows: its rows first, then the waves
+    if (tx <= kWave / 2 && (tx & (tx - 1)) == 0) {                     // a wave holds whole rows: its rows first, then the waves
         const int waves = threads / kWave;
-        for (int o = tx; o < kWave; o <<= 1) {
 #pragma unroll
-            for (int w = 0; w < W; ++w) a[w] += __shfl_xor(a[w], o, kWave);
-        }
+        for (int w = 0; w < W; ++w) a[w] = gn_wave_columns(a[w], tx);
         if (lane_id() < tx) {
 #pragma unroll
             for (int w = 0; w < W; ++w) lds[(w * waves + t / kWave) * tx + lane_id()] = a[w];
@@ -201,6 +240,7 @@ __device__ __forceinline__ void gn_sum_rows(S (&a)[W], int tx, int ty, int row, 
         for (int k = t; k < W * tx; k += threads) {
             const int w = k / tx, col = k - w * tx;
             S sum = lds[(w * waves) * tx + col];
+#pragma unroll 4
             for (int v = 1; v < waves; ++v) sum += lds[(w * waves + v) * tx + col];
             res[k] = sum;
         }
@@ -235,9 +275,9 @@ template <typename F> __device__ __forceinline__ void gn_each_group(int groups, 
 }
 __device__ __forceinline__ double gn_lanes_sum(double v, int lanes) { return lanes == 1 ? v : wave_sum(v); }
 
-__device__ __forceinline__ double2 gn_statistics(double sum, double sq, double m, double eps) {
-    const double mean = sum / m;
-    double var = sq / m - mean * mean;
+__device__ __forceinline__ double2 gn_statistics(double sum, double sq, double inv_m, double eps) {
+    const double mean = sum * inv_m;
+    double var = sq * inv_m - mean * mean;
     var = var < 0.0 ? 0.0 : var;                                       // (NaN stays)
     return make_double2(mean, 1.0 / sqrt(var + eps));
 }
@@ -254,13 +294,13 @@ struct GnSlab {
     int n, c0, groups;
     bool live;
     template <int V> __device__ __forceinline__ void set(const GnShape& s) {
-        const int slabs = s.c / s.cs, b = gn_spread(blockIdx.x, gridDim.x);
-        n = b / slabs;
-        c0 = (b - n * slabs) * s.cs;
-        groups = s.cs / s.cg;
-        tx = s.cs / V;
-        ty = blockDim.x / tx;
-        row = threadIdx.x / tx;
+        const int b = gn_spread(blockIdx.x, gridDim.x);
+        n = b / s.slabs;
+        c0 = (b - n * s.slabs) * s.cs;
+        groups = s.slab_groups;
+        tx = s.tx;
+        ty = s.ty;
+        row = (int)((threadIdx.x * s.tx_inverse) >> 20);
         col = (threadIdx.x - row * tx) * V;
         live = row < ty;
     }
@@ -284,6 +324,8 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_forward_kernel
         const int r = l.row + u * l.ty;
         if (l.live && r < rows) v[u] = gn_read<T, V>(x + base + (int64_t)r * s.c);
     }
+    GnScale<V> ch;
+    ch.weights(w, l.c0 + (l.live ? l.col : 0));
     double a[2] = {0.0, 0.0};
 #pragma unroll
     for (int u = 0; u < R; ++u)
@@ -306,14 +348,13 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_forward_kernel
         sum = gn_lanes_sum(sum, lanes);
         sq = gn_lanes_sum(sq, lanes);
         if (lane == 0) {
-            group[g] = gn_statistics(sum, sq, (double)s.rows * s.cg, eps);
+            group[g] = gn_statistics(sum, sq, s.inv_m, eps);
             stats[(int64_t)l.n * s.groups + l.c0 / s.cg + g] = group[g];
         }
     });
     __syncthreads();
     if (!l.live) return;
-    GnScale<V> ch;
-    ch.load(group[l.col / s.cg], w, l.c0 + l.col);
+    ch.statistics(group[l.col / s.cg]);
     gn_by_act(act, [&](auto A) {
 #pragma unroll
         for (int u = 0; u < R; ++u) {
@@ -390,8 +431,7 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_backward_kerne
         }
         s1 = gn_lanes_sum(s1, lanes);
         s2 = gn_lanes_sum(s2, lanes);
-        const double m = (double)s.rows * s.cg;
-        if (lane == 0) group[g] = make_float2((float)(s1 / m), (float)(s2 / m));
+        if (lane == 0) group[g] = make_float2((float)(s1 * s.inv_m), (float)(s2 * s.inv_m));
     });
     __syncthreads();
     if (!l.live) return;
@@ -498,7 +538,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const double2* __r
     }
     sum = wave_sum(sum);
     sq = wave_sum(sq);
-    if (lane_id() == 0) stats[at] = gn_statistics(sum, sq, (double)s.rows * s.cg, eps);
+    if (lane_id() == 0) stats[at] = gn_statistics(sum, sq, s.inv_m, eps);
 }
 
 template <typename T, int V>
@@ -512,7 +552,8 @@ __global__ __launch_bounds__(kGnThreads) void gn_forward_kernel(const T* __restr
         const GnLanes l = gn_lanes<V>(s.c, tile);
         if (!l.live) continue;
         GnScale<V> ch;
-        ch.load(stats[(int64_t)n * s.groups + l.col / s.cg], w, l.col);
+        ch.weights(w, l.col);
+        ch.statistics(stats[(int64_t)n * s.groups + l.col / s.cg]);
         gn_by_act(act, [&](auto A) {
             gn_rows<T, V, gn_unroll<T, V>()>(x + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, int64_t r) {
                 float o[V];
@@ -626,8 +667,7 @@ __global__ __launch_bounds__(kGnStatThreads) void gn_grad_stats_kernel(const flo
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int k = 1; k < kGnStatThreads / kWave; ++k) { s1 += lds[k].x; s2 += lds[k].y; }
-        const double m = (double)s.rows * s.cg;
-        means[(int64_t)n * s.groups + g] = make_float2((float)(s1 / m), (float)(s2 / m));
+        means[(int64_t)n * s.groups + g] = make_float2((float)(s1 * s.inv_m), (float)(s2 * s.inv_m));
     }
 }
 
@@ -703,11 +743,13 @@ static int gn_vector(int cg, int most) {           // channels of a thread, all 
 static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype, bool backward) {
     GnShape s;
     s.n = n; s.rows = rows; s.c = c; s.groups = groups; s.cg = c / groups;
+    s.inv_m = 1.0 / ((double)rows * s.cg);
     const int item = dtype == GEOMAE_DTYPE_F32 ? 4 : 2;
     // resident, if all rows of a group fit; more groups to a workgroup while its piece of a row is short of a cache line and there
     // are workgroups for every CU without
     s.v = gn_vector(s.cg, 4);
-    s.cs = s.threads = 0;
+    s.cs = s.threads = s.tx = s.ty = s.slabs = s.slab_groups = 0;
+    s.tx_inverse = 0;
     const int held = gn_vectors_held(s.v, item);
     auto fits = [&](int64_t cs) {
         const int64_t tx = cs / s.v;
@@ -724,6 +766,8 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
         threads = threads > kGnResidentThreads ? kGnResidentThreads : threads;
         while (threads < tx || threads / tx * held < rows) threads += kWave;
         s.threads = (int32_t)threads;
+        s.tx = (int32_t)tx; s.ty = (int32_t)(threads / tx); s.slabs = groups / k; s.slab_groups = k;
+        s.tx_inverse = (uint32_t)(((1 << 20) + tx - 1) / tx);
     } else if (!backward && item == 2) s.v = gn_vector(s.cg, 8);
     const int cv = c / s.v, ty = cv < kGnThreads ? kGnThreads / cv : 1, unroll = 64 / (s.v * item) < 16 ? 64 / (s.v * item) : 16;
     const int64_t least = (int64_t)ty * unroll, wanted = kGnBlocks / n > 1 ? kGnBlocks / n : 1;
@@ -823,7 +867,7 @@ extern "C" int geomae_group_norm_forward(const void* x, int32_t dtype, int32_t n
     if (s.cs) {
         gn_by_type<4>(dtype, s.v, [&](auto t, auto vec) {
             typedef typename decltype(t)::type T;
-            hipLaunchKernelGGL((gn_resident_forward_kernel<T, decltype(vec)::value>), dim3(n * (c / s.cs)), dim3(s.threads), gn_resident_lds(s, false), stream,
+            hipLaunchKernelGGL((gn_resident_forward_kernel<T, decltype(vec)::value>), dim3(n * s.slabs), dim3(s.threads), gn_resident_lds(s, false), stream,
                                static_cast<const T*>(x), s, w, eps, activation, static_cast<T*>(y), st);
         });
         return check_launch("gn_resident_forward_kernel");
@@ -859,7 +903,7 @@ extern "C" int geomae_group_norm_backward(const void* x, const void* dy, int32_t
         constexpr int V = decltype(vec)::value;
         const T *in = static_cast<const T*>(x), *grad = static_cast<const T*>(dy);
         if (s.cs) {
-            hipLaunchKernelGGL((gn_resident_backward_kernel<T, V>), dim3(n * (c / s.cs)), dim3(s.threads), gn_resident_lds(s, true), stream, in, grad, s,
+            hipLaunchKernelGGL((gn_resident_backward_kernel<T, V>), dim3(n * s.slabs), dim3(s.threads), gn_resident_lds(s, true), stream, in, grad, s,
                                st, w, activation, static_cast<T*>(dx), n == 1 ? nullptr : ws.channel, dgamma, dbeta);
             if (weights && n > 1) gn_launch_weight_grad(ws.channel, n, s, ws, weight_dtype, dgamma, dbeta, stream);
             return;

@@ -4,6 +4,7 @@
 // entry points bind() takes by address.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include "../../include/geomae_hip.h"
 
@@ -39,12 +40,14 @@ struct AdamwPlan {
     float* norm_word;
     int state_bits;
     uint32_t seed;
+    bool captured;                                                     // a captured step has these addresses
     std::vector<const void*> grads;
     std::vector<int32_t> hyper_of;
+    std::vector<c10::TensorImpl*> changed;
 };
 
-bool same_layout(const at::Tensor& a, const at::Tensor& b) {
-    if (a.sizes() != b.sizes()) return false;
+bool same_layout(const at::Tensor& a, const at::Tensor& b) {         // (of the same sizes)
+    if (a.strides() == b.strides()) return true;
     for (int64_t d = 0; d < a.dim(); ++d)
         if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
     return true;
@@ -94,7 +97,9 @@ bool same_hyper(const GeomaeAdamwHyper& a, const GeomaeAdamwHyper& b) {
 // true: the step is enqueued; false: a parameter is not where the table says (nothing was done)
 bool adamw_step(AdamwPlan& plan, py::list groups, double max_norm, double grad_scale, const c10::optional<at::Tensor>& scale_tensor,
                 bool skip_nonfinite) {
+    const at::NoGradGuard no_grad;
     const size_t n = plan.where.size();
+    plan.changed.clear();
     std::vector<GeomaeAdamwHyper> hypers;
     std::vector<at::Tensor> copies;
     c10::optional<c10::Device> device;
@@ -132,6 +137,7 @@ bool adamw_step(AdamwPlan& plan, py::list groups, double max_norm, double grad_s
                 copies.push_back(at::empty_strided(p.sizes(), p.strides(), p.options()).copy_(grad));
                 plan.grads[i] = copies.back().const_data_ptr();
             }
+            if (plan.grads[i] && !p.is_inference()) plan.changed.push_back(p.unsafeGetTensorImpl());
         }
     }
     if (i != n) return false;
@@ -147,14 +153,8 @@ bool adamw_step(AdamwPlan& plan, py::list groups, double max_norm, double grad_s
                                (int32_t)hypers.size(), plan.state_bits, max_norm, grad_scale, scale_ptr, skip_nonfinite, plan.seed,
                                max_norm > 0.0 || skip_nonfinite ? plan.norm_word : nullptr, plan.workspace, plan.workspace_bytes, stream_of(*device)),
           "geomae_multi_adamw_step");
-    i = 0;
-    for (py::handle g : groups) {                                      // the parameters changed, for autograd's saved tensors too
-        PyObject* list = PyDict_GetItemString(g.ptr(), "params");
-        for (Py_ssize_t j = 0; j < PyList_GET_SIZE(list); ++j, ++i) {
-            const at::Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(list, j));
-            if (plan.grads[i] && !p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
-        }
-    }
+    for (c10::TensorImpl* t : plan.changed) t->bump_version();         // the parameters changed, for autograd's saved tensors too
+    plan.captured = plan.captured || c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
     return true;
 }
 
@@ -330,11 +330,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             p.norm_word = reinterpret_cast<float*>(norm_word);
             p.state_bits = state_bits;
             p.seed = 0;
+            p.captured = false;
             p.grads.resize(where.size());
             p.hyper_of.resize(where.size());
             return p;
         }))
         .def_readwrite("seed", &AdamwPlan::seed)
+        .def_readonly("captured", &AdamwPlan::captured)
         .def("step", &adamw_step);
     m.def("group_norm_act", &group_norm_act);
 }

@@ -51,7 +51,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         self.state_bits, self.master_weights, self.seed = int(state_bits), bool(master_weights), int(seed)
         if not 0 <= self.seed < 2 ** 32:
             raise ValueError("seed must be in [0, 2**32)")
-        self._arena, self._table, self._building, self._captured, self._retired = None, None, True, False, []
+        self._arena, self._table, self._building, self._plan, self._retired = None, None, True, None, []
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         self._building = False
@@ -146,7 +146,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
 
     def _retire(self):
         """What a captured step may still read and write is kept as long as this optimizer."""
-        if self._captured:
+        if self._plan is not None and self._plan.captured:
             self._retired.append((self._table, self._arena, self._chunks, self._workspace, self._norm_word))
 
     @staticmethod
@@ -188,7 +188,6 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                                            self._workspace.data_ptr(), self._workspace.numel(), self._norm_word.data_ptr(), self.state_bits)
 
     # ------------------------------------------------------------------------------------------------ the step
-    @torch.no_grad()
     def step(self, closure=None, max_norm=0.0, grad_scale=1.0, skip_nonfinite=False):
         """One update of every parameter that has a gradient.  max_norm > 0 clips the gradients to that norm over all of
         them (torch.nn.utils.clip_grad_norm_; infinity: only the norm is wanted); grad_scale (a number, or one float32 value on the GPU) multiplies them first;
@@ -202,7 +201,6 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         scale, scale_tensor = (1.0, grad_scale) if torch.is_tensor(grad_scale) else (float(grad_scale), None)
         max_norm = float(max_norm or 0.0)
         self._plan.seed = self.seed
-        self._captured = self._captured or torch.cuda.is_current_stream_capturing()
         if not self._plan.step(self.param_groups, max_norm, scale, scale_tensor, skip_nonfinite):
             self._find_params()
             self._plan.step(self.param_groups, max_norm, scale, scale_tensor, skip_nonfinite)
