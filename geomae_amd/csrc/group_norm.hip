@@ -17,6 +17,8 @@
 //            gradients if there is more than one sample).  Bound by launch, load latency and the workgroup's reductions.
 //  streamed  three launches a pass: sums over a chunk of rows, one value per (sample, group) from the chunks' sums, and the pass
 //            that writes.  Bound by HBM, or the 256 MB cache that the second read of x and dy comes from where they fit in it.
+//            Tensors over 64 MB: the writing pass loads and stores past the caches (4 x 128 x 200 x 200 fp32, both passes 132 ->
+//            117 us; 61 M bf16 elements forward 84 -> 67 us); smaller ones stay there for whoever comes next.
 #include "common.h"
 #include "../../include/geomae_hip.h"
 #include <math.h>
@@ -37,6 +39,7 @@ struct GnShape {
     int32_t n, c, groups, cg;
     int32_t chunks;                                // of a sample's rows (streamed)
     int64_t chunk_rows;
+    int32_t past_cache;                            // streamed: the tensors do not fit the 256 MB cache beside each other
     double inv_m;                                  // 1 / (elements of a group of a sample)
     int32_t v;                                     // channels of a thread
     int32_t cs, threads;                           // channels of a resident workgroup, 0: streamed; its threads ...
@@ -48,14 +51,21 @@ template <typename T> __device__ __forceinline__ float gn_float(T x) { return (f
 template <> __device__ __forceinline__ float gn_float<uint16_t>(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }   // bf16
 // (element-aligned: a tensor may start anywhere, and global memory takes wide accesses at any element's address)
 template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) GnPack { T v[V]; };
-template <typename T, int V> __device__ __forceinline__ GnPack<T, V> gn_read(const T* p) { return *reinterpret_cast<const GnPack<T, V>*>(p); }
+// LAST: the last use of the data for now (GnShape::past_cache): a load and a store that leave the caches to others
+template <typename T, int V> struct GnWords { typedef uint32_t type __attribute__((ext_vector_type(V * sizeof(T) / 4), aligned(sizeof(T)))); };
+template <typename T, int V, bool LAST = false> __device__ __forceinline__ GnPack<T, V> gn_read(const T* p) {
+    if constexpr (LAST && V * sizeof(T) >= 4) {
+        typedef typename GnWords<T, V>::type W;
+        return __builtin_bit_cast(GnPack<T, V>, __builtin_nontemporal_load(reinterpret_cast<const W*>(p)));
+    } else return *reinterpret_cast<const GnPack<T, V>*>(p);
+}
 typedef __bf16 GnBf2 __attribute__((ext_vector_type(2)));
 typedef float GnF2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t gn_bf16_pair(float a, float b) {
     const GnBf2 r = __builtin_convertvector((GnF2){a, b}, GnBf2);
     return __builtin_bit_cast(uint32_t, r);
 }
-template <typename T, int V> __device__ __forceinline__ void gn_write(T* p, const float (&x)[V]) {
+template <typename T, int V, bool LAST = false> __device__ __forceinline__ void gn_write(T* p, const float (&x)[V]) {
     GnPack<T, V> w;
     if constexpr (std::is_same<T, uint16_t>::value) {
 #pragma unroll
@@ -69,7 +79,10 @@ template <typename T, int V> __device__ __forceinline__ void gn_write(T* p, cons
 #pragma unroll
         for (int i = 0; i < V; ++i) w.v[i] = (T)x[i];
     }
-    *reinterpret_cast<GnPack<T, V>*>(p) = w;
+    if constexpr (LAST && V * sizeof(T) >= 4) {
+        typedef typename GnWords<T, V>::type W;
+        __builtin_nontemporal_store(__builtin_bit_cast(W, w), reinterpret_cast<W*>(p));
+    } else *reinterpret_cast<GnPack<T, V>*>(p) = w;
 }
 // vectors that a thread has in flight (streamed; 64 bytes) or holds (resident)
 template <typename T, int V> constexpr int gn_unroll() { return 64 / (int)(V * sizeof(T)) < 16 ? 64 / (int)(V * sizeof(T)) : 16; }
@@ -114,6 +127,12 @@ template <typename F> __host__ __device__ __forceinline__ void gn_by_act(int act
     else if (act == kGnSilu) f(std::integral_constant<int, kGnSilu>());
     else if (act == kGnGelu) f(std::integral_constant<int, kGnGelu>());
     else f(std::integral_constant<int, kGnNone>());
+}
+template <typename F> __device__ __forceinline__ void gn_by_act(int act, int last, F f) {
+    gn_by_act(act, [&](auto a) {
+        if (last) f(a, std::true_type());
+        else f(a, std::false_type());
+    });
 }
 // z > 0 as a comparison of sign * x with a threshold
 __device__ __forceinline__ void gn_threshold(double mean, double scale, double beta, float& sign, float& thr) {
@@ -472,12 +491,12 @@ template <int V> __device__ __forceinline__ GnLanes gn_lanes(int c, int tile) {
     return l;
 }
 // f(vectors of up to U rows, how many): the lane's rows of [r0, r1), U loads at a time
-template <typename T, int V, int U, typename F> __device__ __forceinline__ void gn_rows(const T* x, int c, const GnLanes& l, int64_t r0, int64_t r1, F f) {
+template <typename T, int V, int U, bool LAST = false, typename F> __device__ __forceinline__ void gn_rows(const T* x, int c, const GnLanes& l, int64_t r0, int64_t r1, F f) {
     for (int64_t r = r0 + l.row; r < r1; r += U * l.ty) {
         GnPack<T, V> w[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (r + u * l.ty < r1) w[u] = gn_read<T, V>(x + (r + u * l.ty) * c + l.col);
+            if (r + u * l.ty < r1) w[u] = gn_read<T, V, LAST>(x + (r + u * l.ty) * c + l.col);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (r + u * l.ty < r1) f(w[u], r + u * l.ty);
@@ -554,27 +573,28 @@ __global__ __launch_bounds__(kGnThreads) void gn_forward_kernel(const T* __restr
         GnScale<V> ch;
         ch.weights(w, l.col);
         ch.statistics(stats[(int64_t)n * s.groups + l.col / s.cg]);
-        gn_by_act(act, [&](auto A) {
-            gn_rows<T, V, gn_unroll<T, V>()>(x + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, int64_t r) {
+        gn_by_act(act, s.past_cache, [&](auto A, auto last) {
+            constexpr bool LAST = decltype(last)::value;
+            gn_rows<T, V, gn_unroll<T, V>(), LAST>(x + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, int64_t r) {
                 float o[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) o[i] = ch.template value<decltype(A)::value>(i, gn_float(v.v[i]));
-                gn_write<T, V>(y + base + r * s.c + l.col, o);
+                gn_write<T, V, LAST>(y + base + r * s.c + l.col, o);
             });
         });
     }
 }
 
 // two tensors at once, half the rows in flight of each
-template <typename T, int V, int U, typename F>
+template <typename T, int V, int U, bool LAST = false, typename F>
 __device__ __forceinline__ void gn_rows2(const T* x, const T* dy, int c, const GnLanes& l, int64_t r0, int64_t r1, F f) {
     for (int64_t r = r0 + l.row; r < r1; r += U * l.ty) {
         GnPack<T, V> w[U], d[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (r + u * l.ty < r1) {
-                w[u] = gn_read<T, V>(x + (r + u * l.ty) * c + l.col);
-                d[u] = gn_read<T, V>(dy + (r + u * l.ty) * c + l.col);
+                w[u] = gn_read<T, V, LAST>(x + (r + u * l.ty) * c + l.col);
+                d[u] = gn_read<T, V, LAST>(dy + (r + u * l.ty) * c + l.col);
             }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -719,8 +739,9 @@ __global__ __launch_bounds__(kGnThreads) void gn_backward_kernel(const T* __rest
         ch.load(stats[(int64_t)n * s.groups + l.col / s.cg], w, act, l.col);
         const float2 mean = means[(int64_t)n * s.groups + l.col / s.cg];
         const float c1 = ch.rstd * mean.x, c2 = ch.rstd * mean.y;
-        gn_by_act(act, [&](auto A) {
-            gn_rows2<T, V, (gn_unroll<T, V>() + 1) / 2>(x + base, dy + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, const GnPack<T, V>& d, int64_t r) {
+        gn_by_act(act, s.past_cache, [&](auto A, auto last) {
+            constexpr bool LAST = decltype(last)::value;
+            gn_rows2<T, V, (gn_unroll<T, V>() + 1) / 2, LAST>(x + base, dy + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, const GnPack<T, V>& d, int64_t r) {
                 float o[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -728,7 +749,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_backward_kernel(const T* __rest
                     ch.template value<decltype(A)::value>(i, gn_float(v.v[i]), gn_float(d.v[i]), xhat, dz);
                     o[i] = ch.dx(i, xhat, dz, c1, c2);
                 }
-                gn_write<T, V>(dx + base + r * s.c + l.col, o);
+                gn_write<T, V, LAST>(dx + base + r * s.c + l.col, o);
             });
         });
     }
@@ -744,6 +765,7 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
     GnShape s;
     s.n = n; s.rows = rows; s.c = c; s.groups = groups; s.cg = c / groups;
     s.inv_m = 1.0 / ((double)rows * s.cg);
+    s.past_cache = (double)n * rows * c * (dtype == GEOMAE_DTYPE_F32 ? 4 : 2) > 64e6;
     const int item = dtype == GEOMAE_DTYPE_F32 ? 4 : 2;
     // resident, if all rows of a group fit; more groups to a workgroup while its piece of a row is short of a cache line and there
     // are workgroups for every CU without
