@@ -767,8 +767,10 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
     s.inv_m = 1.0 / ((double)rows * s.cg);
     s.past_cache = (double)n * rows * c * (dtype == GEOMAE_DTYPE_F32 ? 4 : 2) > 64e6;
     const int item = dtype == GEOMAE_DTYPE_F32 ? 4 : 2;
-    // resident, if all rows of a group fit; more groups to a workgroup while its piece of a row is short of a cache line and there
-    // are workgroups for every CU without
+    // resident, if all rows of a group fit (8 x 512 x 60 x 60 fp32 forward 28 us against 35 streamed, 1 x 256 x 64 x 64 9.5 against
+    // 11.6, 8 x 512 x 20 x 20 6.3 against 11.6); more groups to a workgroup while its piece of a row is short of a cache line and there
+    // are workgroups for every CU without.  Streamed for many rows of under 32 bytes, a fraction of each line that is fetched
+    // (8 x 256 x 90 x 90 fp32 in groups of 4 channels: 42 us resident, 38 streamed; 4 x 128 x 100 x 100 bf16: 19 against 16).
     s.v = gn_vector(s.cg, 4);
     s.cs = s.threads = s.tx = s.ty = s.slabs = s.slab_groups = 0;
     s.tx_inverse = 0;
@@ -777,7 +779,7 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
         const int64_t tx = cs / s.v;
         return tx <= kGnResidentThreads && rows <= kGnResidentThreads / tx * held;
     };
-    if (fits(s.cg)) {
+    if (fits(s.cg) && (rows <= 4096 || (int64_t)s.cg * item >= 32)) {
         int k = 1;
         for (int d = 2; d <= groups && (int64_t)k * s.cg * item < 128; ++d)
             if (groups % d == 0 && fits((int64_t)d * s.cg) && (int64_t)n * (groups / d) >= 256) k = d;

@@ -256,6 +256,8 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         if (again) {
             const auto error = std::make_shared<torch::autograd::DelayedError>("group_norm_act has no second derivative", 3);
             torch::autograd::variable_list three(out.begin(), out.begin() + 3);
+            for (at::Tensor& t : three)
+                if (t.defined()) t = t.detach().set_requires_grad(true);
             three = (*error)(std::move(three));
             for (int i = 0; i < 3; ++i) out[i] = three[i];
         }

@@ -19,7 +19,7 @@ _ZERO_EXPONENT = 16             # exponent byte of a block of zeros
 
 def _dense(t):
     """Non-overlapping and dense in some order of its dimensions (contiguous, channels_last, a transpose of either)."""
-    if t.numel() == 0:
+    if t.numel() == 0 or t.is_contiguous():
         return True
     want = 1
     for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
@@ -251,6 +251,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         for k, v in state.items():
             self._arena[k].copy_(v)
         self._arena["step"].fill_(int(step))
+
+    def __getstate__(self):
+        raise TypeError("a MultiTensorAdamW holds device addresses and cannot be copied or pickled: keep its state_dict()")
 
     def state_dict(self):
         sd = super().state_dict()

@@ -135,3 +135,46 @@ def test_group_norm_model_has_the_gradients_of_its_definition(dev):
     for k in g1:
         # ReLU masks next to zero may differ between two fp32 convolutions: a share of 1e-6 of the elements, in the 2-norm 1e-3
         assert float((g1[k] - g2[k]).norm()) <= (bound + 1e-3) * float(g2[k].norm()), k
+
+
+def test_pretraining_step_with_this_optimizer(dev):
+    """The pre-training model under Trainer(type='MultiTensorAdamW') takes the Python schedule; its first update is FlatAdamW's on the
+    same gradients: both are the same operations in fp32, the two sides' beta weights (1 - 0.9f and fp32(0.1)) differ by 2^-22."""
+    import geomae_amd
+    from geomae_amd.configs import mae_sst_model
+    from geomae_amd.train import Trainer
+    cfg = mae_sst_model(encoder_num_blocks=1, decoder_num_blocks=1)
+    pts = [torch.as_tensor(synth.lidar_frame(11 + i, beams=16, n_az=400), device=dev) for i in range(2)]
+    base = dict(lr=1e-3, betas=(0.9, 0.999), weight_decay=0.05, paramwise_cfg=dict(custom_keys={"norm": dict(decay_mult=0.0)}))
+    torch.manual_seed(0)
+    state = geomae_amd.build_model(cfg).state_dict()
+    ends = []
+    for typ in ("AdamW", "MultiTensorAdamW"):
+        model = geomae_amd.build_model(cfg).to(dev).train()
+        model.load_state_dict(state)
+        tr = Trainer(model, dict(base, type=typ))
+        tr.use_engine = False
+        seen, clip = {}, tr._clip_step
+
+        def tap(*a, tr=tr, seen=seen, clip=clip):
+            seen["grad"], seen["start"] = tr.flat.grad.clone(), tr.flat.flat.clone()
+            return clip(*a)
+        tr._clip_step = tap
+        torch.manual_seed(1)
+        losses, gnorm = tr.train_step(pts)
+        assert all(np.isfinite(float(v)) for v in losses.values()) and np.isfinite(float(gnorm))
+        ends.append((tr, seen))
+    (a, sa), (b, sb) = ends
+    assert b.get_engine() is None and torch.equal(sa["start"], sb["start"])
+    b.flat.flat.copy_(sb["start"])
+    b.flat.grad.copy_(sa["grad"])
+    for v in b.opt.state.values():
+        for t in v.values():
+            t.zero_()
+    b._clip_step(b.grad_clip["max_norm"], 1.0)
+    # per element: h (4 |p| + 40 lr) on each side; the first update is lr g / (|g| + eps sqrt(1 - b2) / g ...), at most lr
+    bound = 2 * 2.0 ** -24 * (4 * sb["start"].abs() + 40 * 1e-3)
+    assert ((a.flat.flat - b.flat.flat).abs() <= bound).all()
+    for tr in (a, b):
+        losses, _ = tr.train_step(pts)
+        assert all(np.isfinite(float(v)) for v in losses.values())

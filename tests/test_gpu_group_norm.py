@@ -209,6 +209,39 @@ def test_any_alignment_and_gradient_layout(dev):
         check(got[k], want[k], k)
 
 
+def test_streamed_past_the_caches_at_any_alignment(dev):
+    """Over 64 MB (the form that loads and stores past the caches), x at an odd element, rows that end inside a tile of loads."""
+    for dtype, shape, groups in ((torch.bfloat16, (1, 72, 701, 701), 9), (torch.float32, (1, 36, 701, 701), 6), (torch.float16, (2, 30, 801, 801), 3)):
+        n, c, h, w = shape
+        _, _, wt, b = make(dev, (1, c, 1, 1), torch.float32)
+        buf = torch.randn(n * c * h * w + 3, device=dev).to(dtype)
+        gbuf = torch.randn(n * c * h * w + 1, device=dev).to(dtype)
+        x, dy = buf[3:].view(n, h, w, c).movedim(-1, 1), gbuf[1:].view(n, h, w, c).movedim(-1, 1)
+        want, got = reference(x, groups, wt, b, 1e-5, "gelu", dy), run_both(x, groups, wt, b, "gelu", dy)
+        for k in want:
+            check(got[k], want[k], (dtype, k))
+
+
+def test_no_second_derivative(dev):
+    from geomae_amd import ops
+    x, dy, w, b = make(dev, (2, 24, 9, 7), torch.float32)
+    x = x.detach().requires_grad_()
+    dx, = torch.autograd.grad(ops.group_norm_act(x, 6, w, b, activation="silu"), x, dy, create_graph=True)
+    check(dx, reference(x.detach(), 6, w, b, 1e-5, "silu", dy)["dx"])
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        dx.sum().backward()
+
+
+def test_input_changed_before_the_backward_pass_is_noticed(dev):
+    from geomae_amd import ops
+    x, dy, w, b = make(dev, (2, 24, 9, 7), torch.float32)
+    w.requires_grad_()
+    y = ops.group_norm_act(x, 6, w, b, activation="silu")
+    x.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
+
+
 def test_empty_batches(dev):
     from geomae_amd import ops
     w, b = torch.ones(8, device=dev, requires_grad=True), torch.zeros(8, device=dev, requires_grad=True)

@@ -417,3 +417,41 @@ def test_refusals(dev):
     with pytest.raises(RuntimeError, match="master_weights"):
         opt.masters()
     assert not base.any()
+
+
+def test_is_not_copied_and_steps_after_hooks(dev):
+    import copy
+    import pickle
+    p = torch.nn.Parameter(torch.ones(40, device=dev))
+    opt = new([p])
+    for f in (copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError, match="state_dict"):
+            f(opt)
+    seen = []
+    opt.register_step_post_hook(lambda *a: seen.append(1))
+    sched = torch.optim.lr_scheduler.LambdaLR(opt, lambda k: 0.5 ** k)
+
+    def closure():
+        opt.zero_grad()
+        loss = (p ** 2).sum()
+        loss.backward()
+        return loss
+    version = p._version
+    assert float(opt.step(closure)) == 40.0 and seen == [1] and p._version > version
+    sched.step()
+    assert opt.param_groups[0]["lr"] == LR / 2
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):   # a step between forward and backward is noticed
+        loss = (p ** 2).sum()
+        opt.step()
+        loss.backward()
+
+
+def test_beta_zero_and_eps_zero(dev):
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.linspace(-1, 1, 70, device=dev))
+        p.grad = torch.linspace(1, 2, 70, device=dev)
+        opt = new([p], betas=(0.0, 0.0), eps=0.0, weight_decay=0.0, state_bits=bits)
+        start = f64(p)
+        opt.step()
+        # m = g, v = g g: the update is lr, within the 12 h of its operations, and p rounds once
+        assert np.abs(f64(p) - (start - LR)).max() <= 12 * H * LR + H
