@@ -93,19 +93,19 @@ static int gn_vectors_held(int v, int item) { return v * item == 16 ? 8 : 16; }
 // memory, the bound (61 M bf16 elements, silu: 85 us).  erf by Abramowitz and Stegun 7.1.26 (off by 1.5e-7 at most, which is
 // 1.3 units of fp32's rounding at 1), whose exponential is also the density of gelu's slope.
 __device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f)); }
-__device__ __forceinline__ float gn_normal_cdf(float z, float& density) {       // density: exp(-z^2 / 2)
-    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
-    density = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
-    const float poly = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
-    const float tail = 0.5f * (poly * t) * density;
-    return z < 0.f ? tail : 1.0f - tail;
+__device__ __forceinline__ float gn_normal_tail(float z, float& density) {      // P(normal > |z|); density: exp(-z^2 / 2)
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
+    density = __builtin_amdgcn_exp2f(z * (z * -0.72134752044448170f));
+    const float poly = fmaf(fmaf(fmaf(fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f), t, 0.5f * 1.421413741f), t, 0.5f * -0.284496736f), t,
+                            0.5f * 0.254829592f);
+    return poly * t * density;
 }
 template <int ACT> __device__ __forceinline__ float gn_act(float z) {
     if constexpr (ACT == kGnRelu) return z < 0.f ? 0.f : z;            // NaN stays
     if constexpr (ACT == kGnSilu) return z * gn_sigmoid(z);
-    if constexpr (ACT == kGnGelu) {
+    if constexpr (ACT == kGnGelu) {                                    // z - z tail above zero, z tail below
         float density;
-        return z * gn_normal_cdf(z, density);
+        return fmaf(-fabsf(z), gn_normal_tail(z, density), fmaxf(z, 0.f));
     }
     return z;
 }
@@ -116,8 +116,8 @@ template <int ACT> __device__ __forceinline__ float gn_slope(float z) {     // (
     }
     if constexpr (ACT == kGnGelu) {
         float density;
-        const float cdf = gn_normal_cdf(z, density);
-        return fmaf(z * 0.39894228040143268f, density, cdf);
+        const float tail = gn_normal_tail(z, density);
+        return fmaf(z * 0.39894228040143268f, density, z < 0.f ? tail : 1.0f - tail);
     }
     return 1.0f;
 }

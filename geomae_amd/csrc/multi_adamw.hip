@@ -4,7 +4,8 @@
 //   p *= 1 - lr wd ;  m += (1 - b1) (g' - m) ;  v = b2 v + (1 - b2) g'^2
 //   p -= lr / (1 - b1^s) * m / (sqrt(v) / sqrt(1 - b2^s) + eps)               s = steps this tensor has taken, kept on the device
 //
-// all in fp32 (the norm's sums in fp64: its rounding would reach every element), operation by operation as in optim.hip.
+// all in fp32 (the norm's sums in fp64: its rounding would reach every element); with 32-bit moments operation by operation as in
+// optim.hip, with 8-bit ones the root and the quotient by the hardware's 1-ulp instructions.
 //
 // 8-bit moments: 32 consecutive elements share an exponent byte E (value = code value * 2^(E - 135); a power of two, so that
 // scaling is exact and a block's re-scaling never re-rounds its other elements).  m: sign, 4 exponent and 3 fraction bits
@@ -48,10 +49,7 @@ template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) 
 template <typename T> __device__ __forceinline__ float ma_float(T x) { return (float)x; }
 template <> __device__ __forceinline__ float ma_float<uint16_t>(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }   // bf16
 template <typename T> __device__ __forceinline__ T ma_narrow(float x) { return (T)x; }
-template <> __device__ __forceinline__ uint16_t ma_narrow<uint16_t>(float x) {                                               // to nearest even
-    const uint32_t b = __float_as_uint(x);
-    return x != x ? (uint16_t)((b >> 16) | 0x40) : (uint16_t)((b + 0x7fff + ((b >> 16) & 1)) >> 16);
-}
+template <> __device__ __forceinline__ uint16_t ma_narrow<uint16_t>(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
 
 // kMaVec elements at offset o of a chunk that has `left` of them; FULL: all of the workgroup's
 template <bool FULL, typename T>
@@ -471,7 +469,8 @@ extern "C" int geomae_multi_adamw_step(const GeomaeAdamwTensor* table, const int
                                        float* grad_norm_out, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
     GEOMAE_REQUIRE(num_tensors >= 0, "multi_adamw_step: negative tensor count");
     if (num_tensors == 0) return GEOMAE_OK;
-    GEOMAE_REQUIRE(table && chunks && first_chunk && grads && hyper_of && hypers && num_hypers > 0, "multi_adamw_step: null argument");
+    GEOMAE_REQUIRE(table && first_chunk && grads && hyper_of && hypers && num_hypers > 0, "multi_adamw_step: null argument");
+    GEOMAE_REQUIRE(chunks || first_chunk[num_tensors] == 0, "multi_adamw_step: null argument");
     GEOMAE_REQUIRE(state_bits == 32 || state_bits == 8, "multi_adamw_step: state_bits must be 8 or 32, got %d", state_bits);
     const MaWorkspace w = ma_workspace(workspace, num_tensors);
     if (!workspace || workspace_bytes < w.bytes) {

@@ -2,9 +2,8 @@
 
 `train.FlatAdamW` updates ONE flat fp32 buffer that every parameter was re-homed into.  This one takes the parameters as they
 are -- fp32, bf16 or fp16, frozen ones among them, convolution weights in channels_last, optionally with fp32 masters behind
-16-bit weights -- and holds their moments in 32 or in 8 bits.  A step is a norm pass (where a norm is wanted), one small launch
-for the per-tensor scalars and one update launch for up to 256 tensors each, whatever the tensors' sizes; step counts live on
-the device, so a captured step goes on counting when it is replayed."""
+16-bit weights -- and holds their moments in 32 or in 8 bits.  Step counts live on the device, so a captured step goes on
+counting when it is replayed."""
 import ctypes
 
 import torch
@@ -30,7 +29,7 @@ def _dense(t):
 
 
 class MultiTensorAdamW(torch.optim.Optimizer):
-    """torch.optim.AdamW's update (decoupled weight decay) of all parameters in two or three launches per 256 tensors.
+    """torch.optim.AdamW's update (decoupled weight decay) of all parameters in two launches per 384 tensors, whatever their sizes.
 
     params: tensors or parameter groups (lr, betas, eps, weight_decay per group); all on one GPU, each dense (in any order of
     its dimensions), float32 / bfloat16 / float16.  A group's lr may be a 0-d float32 tensor on that GPU: a captured step then
@@ -38,7 +37,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     state_bits: 32 = moments in fp32; 8 = one byte per moment and element plus one exponent byte for 32 elements, rounded
     stochastically (reproducibly: a function of seed, parameter index, step and element).  The second moment is held as its root.
     master_weights: keep an fp32 copy of every 16-bit parameter and update that; the parameter is its rounding.  Without
-    it a 16-bit parameter is updated in place and rounded to nearest, as torch.optim.AdamW does.
+    it a 16-bit parameter is updated in place and rounded to nearest, as torch.optim.AdamW does.  Whoever else writes such a
+    parameter (a checkpoint loaded into the model alone) calls sync_masters().
 
     The defaults are the pre-training config's (lr 1e-5, weight_decay 0.05).  Gradients are read where they are when step() is
     called; parameters without one are skipped and do not count the step."""
@@ -74,6 +74,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             if torch.is_tensor(g["lr"]) and (g["lr"].dtype != torch.float32 or g["lr"].numel() != 1 or not g["lr"].is_cuda):
                 raise ValueError("a tensor lr must be one float32 value on the GPU")
             self._check_params(g["params"])
+            self._check_apart()
         except Exception:
             self.param_groups.pop()
             raise
@@ -94,6 +95,11 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             if p.layout != torch.strided or not _dense(p):
                 raise RuntimeError("MultiTensorAdamW: parameters must be dense (no gaps or overlaps between their elements)")
 
+    def _check_apart(self):
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self._params() if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("MultiTensorAdamW: two parameters share memory")
+
     def _params(self):
         return [p for g in self.param_groups for p in g["params"]]
 
@@ -103,9 +109,6 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         self._retire()
         params, old = self._params(), self._arena
         dev = params[0].device
-        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise ValueError("MultiTensorAdamW: two parameters share memory")
         offsets, total = [], 0
         for p in params:
             offsets.append(total)
@@ -203,7 +206,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         self._plan.seed = self.seed
         if not self._plan.step(self.param_groups, max_norm, scale, scale_tensor, skip_nonfinite):
             self._find_params()
-            self._plan.step(self.param_groups, max_norm, scale, scale_tensor, skip_nonfinite)
+            if not self._plan.step(self.param_groups, max_norm, scale, scale_tensor, skip_nonfinite):
+                raise RuntimeError("MultiTensorAdamW: the parameters moved during the step")
         if max_norm > 0.0 or skip_nonfinite:
             self.grad_norm = self._norm_word
         return loss
@@ -216,6 +220,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("MultiTensorAdamW: a parameter's storage moved; take one step outside the capture first")
         self._check_params(params)
+        self._check_apart()
         self._fill_table()
 
     # ------------------------------------------------------------------------------------------------ state
@@ -240,6 +245,13 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise RuntimeError("MultiTensorAdamW: made without master_weights")
         return self._arena["master"]
 
+    @torch.no_grad()
+    def sync_masters(self):
+        """Take the masters from the parameters."""
+        for p in self._params():
+            if "master" in self.state[p]:
+                self.state[p]["master"].copy_(p)
+
     def load_flat_state(self, state, step):
         """Fill the moments (and masters) from flat tensors laid out as moments() and masters() give them -- at 8 bits the codes
         and their exponent bytes -- and set every parameter's step count."""
@@ -262,8 +274,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, sd):
-        """A state_dict of this class with the same state_bits and masters, or (32 bits) one of torch.optim.AdamW; masters
-        that it does not hold are taken from the parameters."""
+        """A state_dict of this class with the same state_bits and masters, or (32 bits) one of torch.optim.AdamW.  Parameters
+        that it has no state of begin anew; masters that it does not hold are taken from the parameters."""
         if int(sd.get("state_bits", 32)) != self.state_bits:
             raise ValueError(f"the state holds moments in {sd.get('state_bits', 32)} bits, this optimizer in {self.state_bits}")
         groups = sd["param_groups"]
@@ -276,7 +288,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         for p, i in zip(params, ids):
             st, mine = sd["state"].get(i), self.state[p]
             if st is None:
-                continue
+                st = {k: torch.full((), _ZERO_EXPONENT if k.endswith("exponent") else 0, dtype=v.dtype).expand(v.shape)
+                      for k, v in mine.items() if k != "master"}
             for k, v in mine.items():
                 if k == "master" and k not in st:
                     todo.append((v, p.detach()))
@@ -292,5 +305,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         for v, x in todo:
             v.copy_(x)
         for g, h in zip(self.param_groups, groups):
+            mine, lr = g["lr"], float(h.get("lr", g["lr"]))
             g.update({k: v for k, v in h.items() if k != "params"})
+            g["lr"] = mine.fill_(lr) if torch.is_tensor(mine) else lr   # (a captured step reads a tensor lr where it is)
         self.seed = int(sd.get("seed", self.seed))

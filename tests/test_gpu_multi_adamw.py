@@ -378,6 +378,58 @@ def test_add_param_group_keeps_the_old_state(dev):
         check(opt, p, before[i], f64(p.grad), i, lr=LR if i < len(params) - 2 else 1e-2)
 
 
+def test_nothing_to_update(dev):
+    """Only empty tensors, or no gradient anywhere: nothing moves, and the norm is 0."""
+    empty = torch.nn.Parameter(torch.zeros(0, 3, device=dev))
+    empty.grad = torch.zeros(0, 3, device=dev)
+    full = torch.nn.Parameter(torch.ones(50, device=dev))
+    for params in ([empty], [full], [empty, full]):
+        opt = new(params, state_bits=8)
+        opt.step()
+        opt._norm_word.fill_(7.0)
+        opt.step(max_norm=1.0)
+        assert float(opt.grad_norm) == 0.0 and (full == 1.0).all() and not opt._arena["step"].any()
+
+
+def test_state_that_is_partly_there_and_masters(dev):
+    """A state_dict without some parameters' state: those begin anew.  A tensor lr stays the tensor it was.  Masters follow a
+    parameter that somebody else wrote once they are told."""
+    params, _ = make(dev, torch.bfloat16, [40, 33])
+    lr = torch.tensor(1e-2, device=dev)
+    opt = new(params, state_bits=8, master_weights=True, lr=lr)
+    for _ in range(2):
+        opt.step()
+    sd = opt.state_dict()
+    sd = {**sd, "state": {0: {k: v.clone() for k, v in sd["state"][0].items()}},
+          "param_groups": [{**sd["param_groups"][0], "lr": torch.tensor(5e-3)}]}
+    opt.step()
+    opt.load_state_dict(sd)
+    assert opt.param_groups[0]["lr"] is lr and abs(float(lr) - 5e-3) < 1e-9
+    a, b = (opt.state[p] for p in params)
+    assert int(a["step"]) == 2 and int(b["step"]) == 0 and not b["exp_avg"].any() and not b["exp_avg_sq"].any()
+    assert all(torch.equal(a[k], v) for k, v in sd["state"][0].items())
+    with torch.no_grad():
+        params[1].fill_(0.5)
+    opt.sync_masters()
+    assert (b["master"] == 0.5).all()
+    before = [snapshot(opt, p) for p in params]
+    opt.step()
+    for i, p in enumerate(params):
+        check(opt, p, before[i], f64(p.grad), i, lr=float(lr))
+
+
+def test_a_refused_group_leaves_the_optimizer_as_it_was(dev):
+    base = torch.zeros(96, device=dev)
+    p, q = torch.nn.Parameter(base[:40]), torch.nn.Parameter(base[32:])
+    opt = new([p])
+    with pytest.raises(ValueError, match="share memory"):
+        opt.add_param_group({"params": [q]})
+    p.grad = torch.ones(40, device=dev)
+    before = snapshot(opt, p)
+    opt.step()
+    check(opt, p, before, f64(p.grad), 0)
+
+
 def test_offsets_past_32_bits(dev):
     """2^31 + 4133 elements (bf16, 8-bit moments): the last ones, which a 32-bit offset would miss, are updated."""
     n = 2 ** 31 + 4133
