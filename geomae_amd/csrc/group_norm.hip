@@ -10,8 +10,9 @@
 // true one.  The rest is fp32; the gradient sums are fp32 within a workgroup's rows and fp64 across workgroups, always in the
 // same order.
 //
-// A thread keeps to one vector of V neighbouring channels of one group (V the largest power of two up to 16 bytes that divides
-// cg; up to 4 where x and dy are both held), so that its statistics, gamma and beta stay in registers.  Two forms:
+// A thread keeps to one vector of V neighbouring channels of one group (V = 4, 2 or 1, whichever divides cg first), so that its
+// statistics, gamma and beta stay in registers.  (8 channels of a 16-bit type, one access of 16 bytes, set up twice as much per
+// thread for half as many rows: 2 x 256 x 128 x 128 bf16 forward 22 us against 17.)  Two forms:
 //  resident  all rows of one or more groups fit a workgroup's registers (128 bytes a thread, 1024 threads: 4096 rows of 32
 //            bytes): x and dy are read once and one launch does a pass (the backward pass one more for the parameters'
 //            gradients if there is more than one sample).  Bound by launch, load latency and the workgroup's reductions.
@@ -84,8 +85,9 @@ template <typename T, int V, bool LAST = false> __device__ __forceinline__ void 
         __builtin_nontemporal_store(__builtin_bit_cast(W, w), reinterpret_cast<W*>(p));
     } else *reinterpret_cast<GnPack<T, V>*>(p) = w;
 }
-// vectors that a thread has in flight (streamed; 64 bytes) or holds (resident)
-template <typename T, int V> constexpr int gn_unroll() { return 64 / (int)(V * sizeof(T)) < 16 ? 64 / (int)(V * sizeof(T)) : 16; }
+// vectors that a thread has in flight (streamed) or holds (resident).  8 of four 16-bit channels in flight instead of 4 cost 10 %
+// (4 x 128 x 200 x 200 bf16, both passes 91 us against 82), 2 of four fp32 channels nothing and 128 bytes 20 %.
+constexpr int gn_rows_in_flight(int v) { return 16 / v; }
 template <typename T, int V> constexpr int gn_held() { return V * sizeof(T) == 16 ? 8 : 16; }
 static int gn_vectors_held(int v, int item) { return v * item == 16 ? 8 : 16; }
 
@@ -517,7 +519,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_sums_kernel(const T* __restrict
         const GnLanes l = gn_lanes<V>(s.c, tile);
         double a[2] = {0.0, 0.0};
         if (l.live)
-            gn_rows<T, V, gn_unroll<T, V>()>(x, s.c, l, r0, r1, [&](const GnPack<T, V>& w, int64_t) {
+            gn_rows<T, V, gn_rows_in_flight(V)>(x, s.c, l, r0, r1, [&](const GnPack<T, V>& w, int64_t) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const double d = (double)gn_float(w.v[i]);
@@ -575,7 +577,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_forward_kernel(const T* __restr
         ch.statistics(stats[(int64_t)n * s.groups + l.col / s.cg]);
         gn_by_act(act, s.past_cache, [&](auto A, auto last) {
             constexpr bool LAST = decltype(last)::value;
-            gn_rows<T, V, gn_unroll<T, V>(), LAST>(x + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, int64_t r) {
+            gn_rows<T, V, gn_rows_in_flight(V), LAST>(x + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, int64_t r) {
                 float o[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) o[i] = ch.template value<decltype(A)::value>(i, gn_float(v.v[i]));
@@ -620,7 +622,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_grad_sums_kernel(const T* __res
             GnGrad<V> ch;
             ch.load(stats[(int64_t)n * s.groups + l.col / s.cg], w, act, l.col);
             gn_by_act(act, [&](auto A) {
-                gn_rows2<T, V, (gn_unroll<T, V>() + 1) / 2>(x + base, dy + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, const GnPack<T, V>& d, int64_t) {
+                gn_rows2<T, V, gn_rows_in_flight(V) / 2>(x + base, dy + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, const GnPack<T, V>& d, int64_t) {
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         float xhat, dz;
@@ -741,7 +743,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_backward_kernel(const T* __rest
         const float c1 = ch.rstd * mean.x, c2 = ch.rstd * mean.y;
         gn_by_act(act, s.past_cache, [&](auto A, auto last) {
             constexpr bool LAST = decltype(last)::value;
-            gn_rows2<T, V, (gn_unroll<T, V>() + 1) / 2, LAST>(x + base, dy + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, const GnPack<T, V>& d, int64_t r) {
+            gn_rows2<T, V, gn_rows_in_flight(V) / 2, LAST>(x + base, dy + base, s.c, l, r0, r1, [&](const GnPack<T, V>& v, const GnPack<T, V>& d, int64_t r) {
                 float o[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -756,22 +758,17 @@ __global__ __launch_bounds__(kGnThreads) void gn_backward_kernel(const T* __rest
 }
 
 // ------------------------------------------------------------------------------------------------ host
-static int gn_vector(int cg, int most) {           // channels of a thread, all of one group
-    for (int v = most; v > 1; v >>= 1)
-        if (cg % v == 0) return v;
-    return 1;
-}
-static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype, bool backward) {
+static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype) {
     GnShape s;
     s.n = n; s.rows = rows; s.c = c; s.groups = groups; s.cg = c / groups;
     s.inv_m = 1.0 / ((double)rows * s.cg);
+    s.v = s.cg % 4 == 0 ? 4 : (s.cg % 2 == 0 ? 2 : 1);
     s.past_cache = (double)n * rows * c * (dtype == GEOMAE_DTYPE_F32 ? 4 : 2) > 64e6;
     const int item = dtype == GEOMAE_DTYPE_F32 ? 4 : 2;
     // resident, if all rows of a group fit (8 x 512 x 60 x 60 fp32 forward 28 us against 35 streamed, 1 x 256 x 64 x 64 9.5 against
     // 11.6, 8 x 512 x 20 x 20 6.3 against 11.6); more groups to a workgroup while its piece of a row is short of a cache line and there
     // are workgroups for every CU without.  Streamed for many rows of under 32 bytes, a fraction of each line that is fetched
     // (8 x 256 x 90 x 90 fp32 in groups of 4 channels: 42 us resident, 38 streamed; 4 x 128 x 100 x 100 bf16: 19 against 16).
-    s.v = gn_vector(s.cg, 4);
     s.cs = s.threads = s.tx = s.ty = s.slabs = s.slab_groups = 0;
     s.tx_inverse = 0;
     const int held = gn_vectors_held(s.v, item);
@@ -792,8 +789,8 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
         s.threads = (int32_t)threads;
         s.tx = (int32_t)tx; s.ty = (int32_t)(threads / tx); s.slabs = groups / k; s.slab_groups = k;
         s.tx_inverse = (uint32_t)(((1 << 20) + tx - 1) / tx);
-    } else if (!backward && item == 2) s.v = gn_vector(s.cg, 8);
-    const int cv = c / s.v, ty = cv < kGnThreads ? kGnThreads / cv : 1, unroll = 64 / (s.v * item) < 16 ? 64 / (s.v * item) : 16;
+    }
+    const int cv = c / s.v, ty = cv < kGnThreads ? kGnThreads / cv : 1, unroll = gn_rows_in_flight(s.v);
     const int64_t least = (int64_t)ty * unroll, wanted = kGnBlocks / n > 1 ? kGnBlocks / n : 1;
     s.chunk_rows = (rows + wanted - 1) / wanted;
     s.chunk_rows = s.chunk_rows < least ? least : (s.chunk_rows + least - 1) / least * least;
@@ -848,18 +845,15 @@ static void gn_launch_weight_grad(const double2* channel, int rows, const GnShap
 
 // f(type, vector) for the run-time choice of the two
 template <typename T> struct GnType { typedef T type; };
-template <typename T, int MOST, typename F> static void gn_by_vector(int v, F f) {
-    if constexpr (MOST == 8) {
-        if (v == 8) return f(GnType<T>(), std::integral_constant<int, 8>());
-    }
+template <typename T, typename F> static void gn_by_vector(int v, F f) {
     if (v == 4) f(GnType<T>(), std::integral_constant<int, 4>());
     else if (v == 2) f(GnType<T>(), std::integral_constant<int, 2>());
     else f(GnType<T>(), std::integral_constant<int, 1>());
 }
-template <int MOST16, typename F> static void gn_by_type(int dtype, int v, F f) {
-    if (dtype == GEOMAE_DTYPE_F32) gn_by_vector<float, 4>(v, f);
-    else if (dtype == GEOMAE_DTYPE_BF16) gn_by_vector<uint16_t, MOST16>(v, f);
-    else gn_by_vector<_Float16, MOST16>(v, f);
+template <typename F> static void gn_by_type(int dtype, int v, F f) {
+    if (dtype == GEOMAE_DTYPE_F32) gn_by_vector<float>(v, f);
+    else if (dtype == GEOMAE_DTYPE_BF16) gn_by_vector<uint16_t>(v, f);
+    else gn_by_vector<_Float16>(v, f);
 }
 
 }  // namespace geomae
@@ -869,7 +863,7 @@ using namespace geomae;
 extern "C" int64_t geomae_group_norm_workspace_bytes(int32_t n, int64_t rows, int32_t c, int32_t groups, int32_t dtype, int32_t backward) {
     if (gn_check("group_norm_workspace_bytes", n, rows, c, groups, dtype, 0, 0)) return -1;
     if (n == 0 || rows == 0) return 0;
-    const GnWorkspace w = gn_workspace(nullptr, gn_shape(n, rows, c, groups, dtype, backward != 0));
+    const GnWorkspace w = gn_workspace(nullptr, gn_shape(n, rows, c, groups, dtype));
     return backward ? w.backward_bytes : w.forward_bytes;
 }
 
@@ -880,7 +874,7 @@ extern "C" int geomae_group_norm_forward(const void* x, int32_t dtype, int32_t n
     GEOMAE_REQUIRE(eps >= 0.0, "group_norm_forward: eps must not be negative");
     if (n == 0 || rows == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(x && y && stats, "group_norm_forward: null argument");
-    const GnShape s = gn_shape(n, rows, c, groups, dtype, false);
+    const GnShape s = gn_shape(n, rows, c, groups, dtype);
     const GnWorkspace ws = gn_workspace(workspace, s);
     if (workspace_bytes < ws.forward_bytes || (ws.forward_bytes && !workspace)) {
         set_error("group_norm_forward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws.forward_bytes);
@@ -889,14 +883,14 @@ extern "C" int geomae_group_norm_forward(const void* x, int32_t dtype, int32_t n
     double2* st = reinterpret_cast<double2*>(stats);
     const GnWeights w = {gamma, beta, weight_dtype};
     if (s.cs) {
-        gn_by_type<4>(dtype, s.v, [&](auto t, auto vec) {
+        gn_by_type(dtype, s.v, [&](auto t, auto vec) {
             typedef typename decltype(t)::type T;
             hipLaunchKernelGGL((gn_resident_forward_kernel<T, decltype(vec)::value>), dim3(n * s.slabs), dim3(s.threads), gn_resident_lds(s, false), stream,
                                static_cast<const T*>(x), s, w, eps, activation, static_cast<T*>(y), st);
         });
         return check_launch("gn_resident_forward_kernel");
     }
-    gn_by_type<8>(dtype, s.v, [&](auto t, auto vec) {
+    gn_by_type(dtype, s.v, [&](auto t, auto vec) {
         typedef typename decltype(t)::type T;
         constexpr int V = decltype(vec)::value;
         const T* in = static_cast<const T*>(x);
@@ -913,7 +907,7 @@ extern "C" int geomae_group_norm_backward(const void* x, const void* dy, int32_t
     if (int rc = gn_check("group_norm_backward", n, rows, c, groups, dtype, weight_dtype, activation)) return rc;
     if (n == 0 || rows == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(x && dy && stats && dx, "group_norm_backward: null argument");
-    const GnShape s = gn_shape(n, rows, c, groups, dtype, true);
+    const GnShape s = gn_shape(n, rows, c, groups, dtype);
     const GnWorkspace ws = gn_workspace(workspace, s);
     if (workspace_bytes < ws.backward_bytes || (ws.backward_bytes && !workspace)) {
         set_error("group_norm_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws.backward_bytes);
@@ -922,7 +916,7 @@ extern "C" int geomae_group_norm_backward(const void* x, const void* dy, int32_t
     const double2* st = reinterpret_cast<const double2*>(stats);
     const GnWeights w = {gamma, beta, weight_dtype};
     const bool weights = dgamma || dbeta, many = n > kGnFold;
-    gn_by_type<4>(dtype, s.v, [&](auto t, auto vec) {
+    gn_by_type(dtype, s.v, [&](auto t, auto vec) {
         typedef typename decltype(t)::type T;
         constexpr int V = decltype(vec)::value;
         const T *in = static_cast<const T*>(x), *grad = static_cast<const T*>(dy);
