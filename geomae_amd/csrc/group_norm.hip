@@ -826,7 +826,7 @@ static int gn_check(const char* what, int32_t n, int64_t rows, int32_t c, int32_
                    (long long)rows, (int)c, (int)groups);
     GEOMAE_REQUIRE(c % groups == 0, "%s: %d channels do not divide into %d groups", what, (int)c, (int)groups);
     GEOMAE_REQUIRE(groups <= kGnMaxGroups, "%s: at most %d groups, got %d", what, kGnMaxGroups, (int)groups);
-    GEOMAE_REQUIRE((int64_t)n * groups <= INT32_MAX && (int64_t)n * kGnBlocks <= INT32_MAX && c <= INT32_MAX / 16, "%s: %d samples of %d groups are too many", what,
+    GEOMAE_REQUIRE((int64_t)n * groups <= INT32_MAX && c <= INT32_MAX / 16, "%s: %d samples of %d groups are too many", what,
                    (int)n, (int)groups);
     GEOMAE_REQUIRE(dtype >= 0 && dtype <= 2 && wdtype >= 0 && wdtype <= 2, "%s: unknown dtype", what);
     GEOMAE_REQUIRE(act >= 0 && act <= 3, "%s: unknown activation %d", what, act);
