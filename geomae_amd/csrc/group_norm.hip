@@ -797,6 +797,14 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
     s.chunks = s.cs ? 0 : (int32_t)((rows + s.chunk_rows - 1) / s.chunk_rows);
     return s;
 }
+// the threads of a launch are counted in 32 bits
+static int gn_check_launches(const char* what, const GnShape& s) {
+    const int64_t main = s.cs ? (int64_t)s.n * s.slabs * s.threads : (int64_t)s.n * s.chunks * kGnThreads;
+    const int64_t means = s.cs ? 0 : (int64_t)s.n * s.groups * kGnStatThreads, fold = ((int64_t)s.n + kGnFold - 1) / kGnFold * s.c;
+    GEOMAE_REQUIRE(main <= UINT32_MAX && means <= UINT32_MAX && fold <= INT32_MAX, "%s: %d samples of %d channels in %d groups are too many", what,
+                   (int)s.n, (int)s.c, (int)s.groups);
+    return GEOMAE_OK;
+}
 static int64_t gn_pad(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 struct GnWorkspace { double2* partial; float2* grad_partial; double2 *channel, *folded; float2* means; int64_t forward_bytes, backward_bytes; };
 static GnWorkspace gn_workspace(void* base, const GnShape& s) {
@@ -863,7 +871,9 @@ using namespace geomae;
 extern "C" int64_t geomae_group_norm_workspace_bytes(int32_t n, int64_t rows, int32_t c, int32_t groups, int32_t dtype, int32_t backward) {
     if (gn_check("group_norm_workspace_bytes", n, rows, c, groups, dtype, 0, 0)) return -1;
     if (n == 0 || rows == 0) return 0;
-    const GnWorkspace w = gn_workspace(nullptr, gn_shape(n, rows, c, groups, dtype));
+    const GnShape s = gn_shape(n, rows, c, groups, dtype);
+    if (gn_check_launches("group_norm_workspace_bytes", s)) return -1;
+    const GnWorkspace w = gn_workspace(nullptr, s);
     return backward ? w.backward_bytes : w.forward_bytes;
 }
 
@@ -875,6 +885,7 @@ extern "C" int geomae_group_norm_forward(const void* x, int32_t dtype, int32_t n
     if (n == 0 || rows == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(x && y && stats, "group_norm_forward: null argument");
     const GnShape s = gn_shape(n, rows, c, groups, dtype);
+    if (int rc = gn_check_launches("group_norm_forward", s)) return rc;
     const GnWorkspace ws = gn_workspace(workspace, s);
     if (workspace_bytes < ws.forward_bytes || (ws.forward_bytes && !workspace)) {
         set_error("group_norm_forward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws.forward_bytes);
@@ -908,6 +919,7 @@ extern "C" int geomae_group_norm_backward(const void* x, const void* dy, int32_t
     if (n == 0 || rows == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(x && dy && stats && dx, "group_norm_backward: null argument");
     const GnShape s = gn_shape(n, rows, c, groups, dtype);
+    if (int rc = gn_check_launches("group_norm_backward", s)) return rc;
     const GnWorkspace ws = gn_workspace(workspace, s);
     if (workspace_bytes < ws.backward_bytes || (ws.backward_bytes && !workspace)) {
         set_error("group_norm_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws.backward_bytes);

@@ -29,9 +29,20 @@ int dtype_code(c10::ScalarType t) {
 }
 
 // ------------------------------------------------------------------------------------------------ AdamW over many tensors
-// What stands between two steps: the addresses of the parameters that the device table was made for, and of the table itself.
+// What stands between two steps: where and how the parameters lie that the device table was made for, and the table's address.
+// (A parameter may be cut or cast where it lies: its address alone does not say that the table still fits.)
+struct AdamwParam {
+    const void* at;
+    c10::ScalarType dtype;
+    c10::SmallVector<int64_t, 5> sizes, strides;
+    explicit AdamwParam(const at::Tensor& p)
+        : at(p.const_data_ptr()), dtype(p.scalar_type()), sizes(p.sizes().begin(), p.sizes().end()), strides(p.strides().begin(), p.strides().end()) {}
+    bool is(const at::Tensor& p) const {
+        return p.const_data_ptr() == at && p.scalar_type() == dtype && p.sizes() == c10::IntArrayRef(sizes) && p.strides() == c10::IntArrayRef(strides);
+    }
+};
 struct AdamwPlan {
-    std::vector<const void*> where;
+    std::vector<AdamwParam> params;
     std::vector<int64_t> first_chunk;
     const GeomaeAdamwTensor* table;
     const int32_t* chunks;
@@ -94,11 +105,11 @@ bool same_hyper(const GeomaeAdamwHyper& a, const GeomaeAdamwHyper& b) {
     return a.lr == b.lr && a.lr_ptr == b.lr_ptr && a.beta1 == b.beta1 && a.beta2 == b.beta2 && a.eps == b.eps && a.weight_decay == b.weight_decay;
 }
 
-// true: the step is enqueued; false: a parameter is not where the table says (nothing was done)
+// true: the step is enqueued; false: a parameter is not where or what the table says (nothing was done)
 bool adamw_step(AdamwPlan& plan, py::list groups, double max_norm, double grad_scale, const c10::optional<at::Tensor>& scale_tensor,
                 bool skip_nonfinite) {
     const at::NoGradGuard no_grad;
-    const size_t n = plan.where.size();
+    const size_t n = plan.params.size();
     plan.changed.clear();
     std::vector<GeomaeAdamwHyper> hypers;
     std::vector<at::Tensor> copies;
@@ -114,7 +125,7 @@ bool adamw_step(AdamwPlan& plan, py::list groups, double max_norm, double grad_s
             PyObject* o = PyList_GET_ITEM(list, j);
             TORCH_CHECK_TYPE(THPVariable_Check(o), "MultiTensorAdamW: a parameter is not a tensor");
             const at::Tensor& p = THPVariable_Unpack(o);
-            if (i >= n || p.const_data_ptr() != plan.where[i]) return false;
+            if (i >= n || !plan.params[i].is(p)) return false;
             if (!device) device = p.device();
             if (k < 0) {
                 const GeomaeAdamwHyper h = hyper_of_group(g.ptr(), *device);
@@ -213,6 +224,21 @@ std::pair<at::Tensor, at::Tensor> group_norm_forward(const at::Tensor& x, const 
     return {y, stats};
 }
 
+// The gradient of a leaf that a graph of eager work on the default stream still holds is accumulated there: while another stream
+// is captured, autograd would order the two streams, which a capture does not survive (it ends the process).
+bool accumulates_on_default_stream(const at::Tensor& t) {
+    if (!t.defined()) return false;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto stream = node ? node->stream() : c10::nullopt;
+    return stream && stream->id() == 0;
+}
+void check_capture(const torch::autograd::variable_list& leaves) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const at::Tensor& t : leaves)
+        TORCH_CHECK(!accumulates_on_default_stream(t), "group_norm_act: a backward pass cannot be captured while a graph of eager work on the "
+                    "default stream holds the gradient of the same leaf: release its outputs first, or do that work on another stream");
+}
+
 struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const c10::optional<at::Tensor>& weight_,
                               const c10::optional<at::Tensor>& bias_, int64_t groups, double eps, int64_t act) {
@@ -232,6 +258,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         {
             at::AutoGradMode off(false);
             const c10::OptionalDeviceGuard guard(x.device());
+            check_capture({x, weight, bias});
             // (needs_input_grad counts the defined tensors among the inputs)
             at::Tensor dweight = weight.defined() && ctx->needs_input_grad(1) ? at::empty_like(weight) : at::Tensor();
             at::Tensor dbias = bias.defined() && ctx->needs_input_grad(2) ? at::empty_like(bias) : at::Tensor();
@@ -319,11 +346,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         }
     });
     py::class_<AdamwPlan>(m, "AdamwPlan")
-        .def(py::init([](const std::vector<uintptr_t>& where, std::vector<int64_t> first_chunk, uintptr_t table, uintptr_t chunks, uintptr_t workspace,
+        .def(py::init([](const std::vector<at::Tensor>& params, std::vector<int64_t> first_chunk, uintptr_t table, uintptr_t chunks, uintptr_t workspace,
                          int64_t workspace_bytes, uintptr_t norm_word, int state_bits) {
-            TORCH_CHECK(first_chunk.size() == where.size() + 1, "AdamwPlan: one first chunk per tensor and the end are wanted");
+            TORCH_CHECK(first_chunk.size() == params.size() + 1, "AdamwPlan: one first chunk per tensor and the end are wanted");
             AdamwPlan p;
-            for (uintptr_t w : where) p.where.push_back(reinterpret_cast<const void*>(w));
+            for (const at::Tensor& t : params) p.params.emplace_back(t);
             p.first_chunk = std::move(first_chunk);
             p.table = reinterpret_cast<const GeomaeAdamwTensor*>(table);
             p.chunks = reinterpret_cast<const int32_t*>(chunks);
@@ -333,12 +360,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             p.state_bits = state_bits;
             p.seed = 0;
             p.captured = false;
-            p.grads.resize(where.size());
-            p.hyper_of.resize(where.size());
+            p.grads.resize(params.size());
+            p.hyper_of.resize(params.size());
             return p;
         }))
         .def_readwrite("seed", &AdamwPlan::seed)
         .def_readonly("captured", &AdamwPlan::captured)
         .def("step", &adamw_step);
     m.def("group_norm_act", &group_norm_act);
+    m.def("accumulates_on_default_stream", &accumulates_on_default_stream);
 }

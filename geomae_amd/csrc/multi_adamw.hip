@@ -471,6 +471,7 @@ extern "C" int geomae_multi_adamw_step(const GeomaeAdamwTensor* table, const int
     if (num_tensors == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(table && first_chunk && grads && hyper_of && hypers && num_hypers > 0, "multi_adamw_step: null argument");
     GEOMAE_REQUIRE(chunks || first_chunk[num_tensors] == 0, "multi_adamw_step: null argument");
+    GEOMAE_REQUIRE(max_norm >= 0.0, "multi_adamw_step: max_norm must not be negative");
     GEOMAE_REQUIRE(state_bits == 32 || state_bits == 8, "multi_adamw_step: state_bits must be 8 or 32, got %d", state_bits);
     const MaWorkspace w = ma_workspace(workspace, num_tensors);
     if (!workspace || workspace_bytes < w.bytes) {

@@ -187,7 +187,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         self._retire()
         self._table = host.to(params[0].device)
         self._layout = [(p.shape, p.stride(), p.dtype, p.device) for p in params]
-        self._plan = _lib.host().AdamwPlan([p.data_ptr() for p in params], self._first_chunk, self._table.data_ptr(), self._chunks.data_ptr(),
+        self._plan = _lib.host().AdamwPlan(params, self._first_chunk, self._table.data_ptr(), self._chunks.data_ptr(),
                                            self._workspace.data_ptr(), self._workspace.numel(), self._norm_word.data_ptr(), self.state_bits)
 
     # ------------------------------------------------------------------------------------------------ the step
@@ -203,6 +203,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                 loss = closure()
         scale, scale_tensor = (1.0, grad_scale) if torch.is_tensor(grad_scale) else (float(grad_scale), None)
         max_norm = float(max_norm or 0.0)
+        if not max_norm >= 0.0:
+            raise ValueError(f"max_norm must not be negative, got {max_norm}")
         self._plan.seed = self.seed
         if not self._plan.step(self.param_groups, max_norm, scale, scale_tensor, skip_nonfinite):
             self._find_params()
@@ -213,7 +215,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         return loss
 
     def _find_params(self):
-        """A parameter is not where the device table says: make the table anew."""
+        """A parameter is not where or what the device table says: make the table anew."""
         params = self._params()
         if [(p.shape, p.stride(), p.dtype, p.device) for p in params] != self._layout:
             raise RuntimeError("MultiTensorAdamW: a parameter changed its shape, layout, dtype or device; make a new optimizer")

@@ -355,3 +355,36 @@ def test_module_and_refusals(dev):
     from geomae_amd._lib import GeomaeLibraryError
     with pytest.raises(GeomaeLibraryError, match="at most 1024"):
         ops.group_norm_act(torch.zeros(1, 2048, device=dev), 2048)
+
+
+def test_capture_beside_a_graph_of_eager_work_is_refused(dev):
+    """A backward pass in a capture, while eager work on the default stream holds the gradient of the same weight, is an error
+    that leaves the process and the stream usable; once that work is released the capture succeeds."""
+    from geomae_amd import _lib, ops
+    on_default = _lib.host().accumulates_on_default_stream
+    x, dy, w, b = make(dev, (2, 16, 8, 8), torch.float32)
+    w, b = w.requires_grad_(), b.requires_grad_()
+    side = torch.cuda.Stream()
+    assert not on_default(w)
+    held = ops.group_norm_act(x, 4, w, b)
+    assert on_default(w) and on_default(b) and not on_default(x) and not on_default(held)
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(graph, stream=side):
+            torch.autograd.grad(ops.group_norm_act(x, 4, w, b), (w, b), dy)
+    del held, graph
+    assert not on_default(w) and not on_default(b)
+    with torch.cuda.stream(side):
+        y = ops.group_norm_act(x, 4, w, b)
+        assert not on_default(w)
+        torch.autograd.grad(y, (w, b), dy)
+        del y
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = torch.autograd.grad(ops.group_norm_act(x, 4, w, b), (w, b), dy)
+    for _ in range(2):
+        graph.replay()
+        want = torch.autograd.grad(ops.group_norm_act(x, 4, w, b), (w, b), dy)
+        assert all(torch.equal(a, c) for a, c in zip(want, got))

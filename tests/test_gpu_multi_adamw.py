@@ -507,3 +507,24 @@ def test_beta_zero_and_eps_zero(dev):
         opt.step()
         # m = g, v = g g: the update is lr, within the 12 h of its operations, and p rounds once
         assert np.abs(f64(p) - (start - LR)).max() <= 12 * H * LR + H
+
+
+def test_a_parameter_changed_where_it_lies_is_refused(dev):
+    """The same address with another length, order or type: no step, nothing changed."""
+    for change in (lambda t: t[:2], lambda t: t.t(), lambda t: t.reshape(-1)):
+        p = torch.nn.Parameter(torch.randn(4, 6, device=dev))
+        other = torch.nn.Parameter(torch.randn(5, device=dev))
+        opt = new([other, p])
+        before = other.detach().clone()
+        p.data = change(p.data)
+        p.grad, other.grad = torch.ones_like(p), torch.ones_like(other)
+        with pytest.raises(RuntimeError, match="shape, layout"):
+            opt.step()
+        assert torch.equal(other, before) and int(opt.state[other]["step"]) == 0
+    opt = new([other])
+    other.grad = torch.ones_like(other)
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            opt.step(max_norm=bad)
+    opt.step(max_norm=None)
+    assert int(opt.state[other]["step"]) == 1

@@ -77,3 +77,14 @@ def test_entry_points_check_their_arguments():
     def backward(dy=64, n=2, bytes_=1 << 20):
         return lib.geomae_group_norm_backward(64, dy, 0, n, rows, 8, 2, None, None, 0, 0, 64, 64, None, None, 64, bytes_, None)
     assert backward(n=0) == 0 and backward(dy=None) < 0 and backward(bytes_=8) == -3
+
+
+def test_more_threads_than_a_launch_counts_are_refused():
+    """Rows [N, C] as samples of one row each: one workgroup of 64 threads for up to 128 bytes of a row."""
+    from geomae_amd import _lib
+    lib = _lib.load()
+    ok = lib.geomae_group_norm_workspace_bytes((1 << 26) - 1, 1, 64, 8, 1, 0)
+    assert ok == 0
+    assert lib.geomae_group_norm_workspace_bytes(1 << 26, 1, 64, 8, 1, 0) == -1 and b"too many" in lib.geomae_last_error()
+    assert lib.geomae_group_norm_forward(64, 1, 1 << 26, 1, 64, 8, None, None, 0, 1e-5, 0, 64, 64, None, 0, None) < 0
+    assert lib.geomae_group_norm_backward(64, 64, 1, 1 << 26, 1, 64, 8, None, None, 0, 0, 64, 64, None, None, None, 0, None) < 0

@@ -102,3 +102,28 @@ def test_entry_points_check_their_arguments():
     assert lib.geomae_adamw_moments8(None, None, None, None, 33, None, None, None) < 0
     assert lib.geomae_adamw_moments8(None, None, None, None, 32, None, None, None) < 0
     assert lib.geomae_adamw_moments8(None, None, None, None, 0, None, None, None) == 0
+
+
+def test_a_plan_notices_a_parameter_cut_or_cast_where_it_lies():
+    """The device table holds lengths: a parameter at the same address but of another size, order or type is not stepped."""
+    from geomae_amd import _lib
+    for change in (lambda t: t[:3], lambda t: t.t(), lambda t: t.view(torch.int32), lambda t: t.reshape(-1), lambda t: t[:1].expand(4, 5)):
+        p = torch.nn.Parameter(torch.zeros(4, 5), requires_grad=False)
+        plan = _lib.host().AdamwPlan([p], [0, 1], 0, 0, 0, 0, 0, 32)
+        where = p.data_ptr()
+        p.data = change(p.data)
+        assert p.data_ptr() == where
+        group = dict(params=[p], lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0)
+        assert plan.step([group], 0.0, 1.0, None, False) is False
+        assert plan.step([dict(group, params=[])], 0.0, 1.0, None, False) is False
+
+
+def test_a_clipping_norm_is_not_negative():
+    import ctypes
+    from geomae_amd import _lib
+    lib = _lib.load()
+    one, grads, which = (ctypes.c_int64 * 2)(0, 1), (ctypes.c_void_p * 1)(64), (ctypes.c_int32 * 1)(0)
+    hypers = (_lib.GeomaeAdamwHyper * 1)()
+    for bad in (-1.0, float("nan")):
+        assert lib.geomae_multi_adamw_step(64, 64, one, 1, grads, which, ctypes.addressof(hypers), 1, 32, bad, 1.0, None, 0, 0, None, None,
+                                           0, None) < 0 and b"max_norm" in lib.geomae_last_error()
