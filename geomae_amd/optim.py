@@ -7,6 +7,7 @@ counting when it is replayed."""
 import ctypes
 
 import torch
+from torch.optim.optimizer import _global_optimizer_post_hooks, _global_optimizer_pre_hooks
 
 from . import _lib
 from .ops import _ptr
@@ -197,6 +198,18 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         skip_nonfinite leaves everything as it was if their norm is not finite.  After a step with max_norm or
         skip_nonfinite, `grad_norm` is the scaled gradients' norm before clipping (a 0-d tensor that the next step
         overwrites).  Gradients are not changed."""
+        # (a class that overrides step() is wrapped itself)
+        if type(self).step is MultiTensorAdamW.step and (
+                self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _global_optimizer_pre_hooks
+                or _global_optimizer_post_hooks or torch.autograd._profiler_enabled()):
+            return self._observed_step(closure, max_norm, grad_scale, skip_nonfinite)
+        return self._step(closure, max_norm, grad_scale, skip_nonfinite)
+
+    # torch wraps step() of every optimizer for hooks and the profiler, 5 us on the host where a step of few tensors takes 9: here
+    # the wrapper is gone through when there is a hook or a profiler
+    step.hooked = True
+
+    def _step(self, closure=None, max_norm=0.0, grad_scale=1.0, skip_nonfinite=False):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -213,6 +226,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if max_norm > 0.0 or skip_nonfinite:
             self.grad_norm = self._norm_word
         return loss
+
+    _observed_step = torch.optim.Optimizer.profile_hook_step(_step)
 
     def _find_params(self):
         """A parameter is not where or what the device table says: make the table anew."""

@@ -528,3 +528,36 @@ def test_a_parameter_changed_where_it_lies_is_refused(dev):
             opt.step(max_norm=bad)
     opt.step(max_norm=None)
     assert int(opt.state[other]["step"]) == 1
+
+
+def test_hooks_profiler_and_subclasses(dev):
+    """Step hooks of the optimizer and of all optimizers run once a step, with the step's arguments, also where a subclass
+    overrides step(); the profiler sees the step."""
+    from geomae_amd.optim import MultiTensorAdamW
+    from torch.optim.optimizer import register_optimizer_step_post_hook, register_optimizer_step_pre_hook
+
+    class Counting(MultiTensorAdamW):
+        def step(self, *args, **kw):
+            self.count = getattr(self, "count", 0) + 1
+            return super().step(*args, **kw)
+    for cls in (MultiTensorAdamW, Counting):
+        p = torch.nn.Parameter(torch.ones(40, device=dev))
+        p.grad = torch.full_like(p, 2.0)
+        opt, seen = cls([p], lr=LR), []
+        handles = [register_optimizer_step_pre_hook(lambda o, a, k: seen.append("all before")),
+                   register_optimizer_step_post_hook(lambda o, a, k: seen.append("all after"))]
+        opt.step()
+        assert seen == ["all before", "all after"]
+        for h in handles:
+            h.remove()
+        opt.step()
+        assert len(seen) == 2 and int(opt.state[p]["step"]) == 2
+        seen.clear()
+        handle = opt.register_step_pre_hook(lambda o, a, k: seen.append(p.grad.mul_(0.5)))
+        opt.step(max_norm=float("inf"))
+        assert len(seen) == 1 and abs(float(opt.grad_norm) - 40 ** 0.5) < 1e-5
+        handle.remove()
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+            opt.step()
+        assert sum(f"Optimizer.step#{cls.__name__}.step" in e.name for e in prof.events()) == 1
+        assert int(opt.state[p]["step"]) == 4 and getattr(opt, "count", 4) == 4
