@@ -85,6 +85,16 @@ template <typename T, int V, bool LAST = false> __device__ __forceinline__ void 
         __builtin_nontemporal_store(__builtin_bit_cast(W, w), reinterpret_cast<W*>(p));
     } else *reinterpret_cast<GnPack<T, V>*>(p) = w;
 }
+// The vector as it is, to the compiler a new one (another one per ACT): its conversions stay where they are used.  Those of all
+// activations' loops were moved ahead of the choice between them, 128 values in fp16, which spilled.
+template <int ACT, typename T, int V> __device__ __forceinline__ GnPack<T, V> gn_fresh(const GnPack<T, V>& p) {
+    if constexpr (V * sizeof(T) >= 4) {
+        struct Words { uint32_t w[V * sizeof(T) / 4]; } words = __builtin_bit_cast(Words, p);
+#pragma unroll
+        for (uint32_t& w : words.w) asm volatile("; %1" : "+v"(w) : "n"(ACT));
+        return __builtin_bit_cast(GnPack<T, V>, words);
+    } else return p;
+}
 // vectors that a thread has in flight (streamed) or holds (resident).  8 of four 16-bit channels in flight instead of 4 cost 10 %
 // (4 x 128 x 200 x 200 bf16, both passes 91 us against 82), 2 of four fp32 channels nothing and 128 bytes 20 %.
 constexpr int gn_rows_in_flight(int v) { return 16 / v; }
@@ -136,18 +146,15 @@ template <typename F> __device__ __forceinline__ void gn_by_act(int act, int las
         else f(a, std::false_type());
     });
 }
-// z > 0 as a comparison of sign * x with a threshold
-__device__ __forceinline__ void gn_threshold(double mean, double scale, double beta, float& sign, float& thr) {
-    sign = scale < 0.0 ? -1.0f : 1.0f;
-    if (scale == 0.0) {
-        thr = beta > 0.0 ? -INFINITY : INFINITY;
-        return;
-    }
-    const double t = (mean - beta / scale) * (double)sign;
+// z > 0 as a comparison of x, its sign turned where gamma is negative, with a threshold
+__device__ __forceinline__ float gn_threshold(double mean, double scale, double beta) {
+    if (scale == 0.0) return beta > 0.0 ? -INFINITY : INFINITY;
+    const double t = scale < 0.0 ? beta / scale - mean : mean - beta / scale;
     float f = (float)t;
     if ((double)f > t) f = nextafterf(f, -INFINITY);
-    thr = f;
+    return f;
 }
+__device__ __forceinline__ float gn_turned(float x, float gamma) { return __uint_as_float(__float_as_uint(x) ^ (__float_as_uint(gamma) & 0x80000000u)); }
 
 __device__ __forceinline__ float gn_weight(const void* w, int dtype, int c, float none) {
     if (!w) return none;
@@ -188,7 +195,7 @@ template <int V> struct GnScale {
 };
 // ... and for xhat and dz
 template <int V> struct GnGrad {
-    float mean, rstd, rest, gamma[V], beta[V], sign[V], thr[V];
+    float mean, rstd, rest, gamma[V], other[V];                       // other: beta; ReLU: gn_threshold
     __device__ __forceinline__ void load(double2 stat, const GnWeights& w, int act, int col) {
         mean = (float)stat.x;
         rstd = (float)stat.y;
@@ -196,14 +203,14 @@ template <int V> struct GnGrad {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             gamma[i] = gn_weight(w.gamma, w.dtype, col + i, 1.f);
-            beta[i] = gn_weight(w.beta, w.dtype, col + i, 0.f);
-            if (act == kGnRelu) gn_threshold(stat.x, stat.y * (double)gamma[i], (double)beta[i], sign[i], thr[i]);
+            other[i] = gn_weight(w.beta, w.dtype, col + i, 0.f);
+            if (act == kGnRelu) other[i] = gn_threshold(stat.x, stat.y * (double)gamma[i], (double)other[i]);
         }
     }
     template <int ACT> __device__ __forceinline__ void value(int i, float x, float dy, float& xhat, float& dz) const {
         xhat = fmaf(x - mean, rstd, rest);
-        if constexpr (ACT == kGnRelu) dz = x * sign[i] > thr[i] ? dy : 0.f;
-        else dz = dy * gn_slope<ACT>(fmaf(xhat, gamma[i], beta[i]));
+        if constexpr (ACT == kGnRelu) dz = gn_turned(x, gamma[i]) > other[i] ? dy : 0.f;
+        else dz = dy * gn_slope<ACT>(fmaf(xhat, gamma[i], other[i]));
     }
     // c1, c2: rstd times the group's two means
     __device__ __forceinline__ float dx(int i, float xhat, float dz, float c1, float c2) const {
@@ -245,11 +252,12 @@ template <typename S> __device__ __forceinline__ S gn_wave_columns(S v, int tx) 
     if (tx <= 1) v += gn_dpp<0x121>(v);
     return v;
 }
+__host__ __device__ __forceinline__ bool gn_whole_rows(int tx) { return tx <= kWave / 2 && (tx & (tx - 1)) == 0; }   // a wave holds whole rows
 // a[W] of every thread (row, col) of tx columns x ty rows, summed over the rows: res[w * tx + col].  Fixed order.
 template <typename S, int W>
-__device__ __forceinline__ void gn_sum_rows(S (&a)[W], int tx, int ty, int row, S* res, S* lds) {
+__device__ __forceinline__ void gn_sum_rows(S (&a)[W], int tx, int ty, S* res, S* lds) {
     const int threads = blockDim.x, t = threadIdx.x;
-    if (tx <= kWave / 2 && (tx & (tx - 1)) == 0) {                     // a wave holds whole rows: its rows first, then the waves
+    if (gn_whole_rows(tx)) {                                           // a wave's rows first, then the waves
         const int waves = threads / kWave;
 #pragma unroll
         for (int w = 0; w < W; ++w) a[w] = gn_wave_columns(a[w], tx);
@@ -268,19 +276,21 @@ __device__ __forceinline__ void gn_sum_rows(S (&a)[W], int tx, int ty, int row, 
     } else {
 #pragma unroll
         for (int w = 0; w < W; ++w) lds[w * threads + t] = a[w];
-        for (int have = ty; have > 1;) {
-            const int half = (have + 1) >> 1;
-            __syncthreads();
-            if (row + half < have) {
-#pragma unroll
-                for (int w = 0; w < W; ++w) lds[w * threads + t] += lds[w * threads + t + half * tx];
-            }
-            have = half;
-        }
         __syncthreads();
-        if (t < tx) {
-#pragma unroll
-            for (int w = 0; w < W; ++w) res[w * tx + t] = lds[w * threads + t];
+        // a row of 16 lanes a column, or a thread if it has few rows
+        const int lanes = ty > 16 ? 16 : 1, lane = t & (lanes - 1);
+        for (int k = t / lanes; k < W * tx; k += threads / lanes) {
+            const int w = k / tx, col = k - w * tx;
+            S sum = 0;
+#pragma unroll 4
+            for (int r = lane; r < ty; r += lanes) sum += lds[w * threads + r * tx + col];
+            if (lanes > 1) {
+                sum += gn_dpp<0x128>(sum);         // row_ror:8
+                sum += gn_dpp<0x124>(sum);
+                sum += gn_dpp<0x122>(sum);
+                sum += gn_dpp<0x121>(sum);
+            }
+            if (lane == 0) res[k] = sum;
         }
     }
     __syncthreads();
@@ -358,7 +368,7 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_forward_kernel
                 a[1] = fma(d, d, a[1]);
             }
         }
-    gn_sum_rows<double, 2>(a, l.tx, l.ty, l.row, res, lds);
+    gn_sum_rows<double, 2>(a, l.tx, l.ty, res, lds);
     const int per = s.cg / V;
     gn_each_group(l.groups, per, [&](int g, int lane, int lanes) {
         double sum = 0.0, sq = 0.0;
@@ -382,8 +392,9 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_forward_kernel
             const int r = l.row + u * l.ty;
             if (r < rows) {
                 float o[V];
+                const GnPack<T, V> xv = gn_fresh<decltype(A)::value>(v[u]);
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = ch.template value<decltype(A)::value>(i, gn_float(v[u].v[i]));
+                for (int i = 0; i < V; ++i) o[i] = ch.template value<decltype(A)::value>(i, gn_float(xv.v[i]));
                 gn_write<T, V>(y + base + (int64_t)r * s.c, o);
             }
         }
@@ -400,7 +411,8 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_backward_kerne
     l.set<V>(s);
     float2* group = reinterpret_cast<float2*>(gn_lds);
     float* res = reinterpret_cast<float*>(group + l.groups);           // [2 V][tx]
-    float* lds = res + 2 * V * l.tx;
+    float* gamma = res + 2 * V * l.tx;                                 // [V][tx], whole rows
+    float* lds = gamma + (gn_whole_rows(l.tx) ? V * l.tx : 0);
     const int64_t base = (int64_t)l.n * s.rows * s.c + l.c0 + l.col;
     const int rows = (int)s.rows;
     GnPack<T, V> v[R], d[R];
@@ -415,24 +427,32 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_backward_kerne
     GnGrad<V> ch;
     const int mine = l.live ? l.col : 0;
     ch.load(stats[(int64_t)l.n * s.groups + (l.c0 + mine) / s.cg], w, act, l.c0 + mine);
-    float a[V], b[V];
+    float ab[2 * V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) a[i] = b[i] = 0.f;
+    for (int i = 0; i < 2 * V; ++i) ab[i] = 0.f;
     gn_by_act(act, [&](auto A) {
 #pragma unroll
         for (int u = 0; u < R; ++u)
             if (l.live && l.row + u * l.ty < rows) {
+                const GnPack<T, V> xv = gn_fresh<decltype(A)::value>(v[u]), dv = gn_fresh<decltype(A)::value>(d[u]);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     float xhat, dz;
-                    ch.template value<decltype(A)::value>(i, gn_float(v[u].v[i]), gn_float(d[u].v[i]), xhat, dz);
-                    a[i] += dz;
-                    b[i] = fmaf(dz, xhat, b[i]);
+                    ch.template value<decltype(A)::value>(i, gn_float(xv.v[i]), gn_float(dv.v[i]), xhat, dz);
+                    ab[i] += dz;
+                    ab[V + i] = fmaf(dz, xhat, ab[V + i]);
                 }
             }
     });
-    gn_sum_rows<float, V>(a, l.tx, l.ty, l.row, res, lds);
-    gn_sum_rows<float, V>(b, l.tx, l.ty, l.row, res + V * l.tx, lds);
+    if (gn_whole_rows(l.tx) && l.live && l.row == 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) gamma[i * l.tx + l.col / V] = ch.gamma[i];
+    }
+    if (l.tx <= kGnResidentThreads / 2) gn_sum_rows<float, 2 * V>(ab, l.tx, l.ty, res, lds);
+    else {                                                             // (64 KB of LDS: half of the sums at a time)
+        gn_sum_rows<float, V>(*reinterpret_cast<float(*)[V]>(&ab[0]), l.tx, l.ty, res, lds);
+        gn_sum_rows<float, V>(*reinterpret_cast<float(*)[V]>(&ab[V]), l.tx, l.ty, res + V * l.tx, lds);
+    }
     for (int c = threadIdx.x; c < s.cs; c += blockDim.x) {
         const int k = c / V, i = c - k * V;
         const float sa = res[i * l.tx + k], sb = res[(V + i) * l.tx + k];
@@ -446,7 +466,7 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_backward_kerne
         double s1 = 0.0, s2 = 0.0;
         for (int c = g * s.cg + lane; c < (g + 1) * s.cg; c += lanes) {
             const int k = c / V, i = c - k * V;
-            const double gm = (double)gn_weight(w.gamma, w.dtype, l.c0 + c, 1.f);
+            const double gm = (double)(gn_whole_rows(l.tx) ? gamma[i * l.tx + k] : gn_weight(w.gamma, w.dtype, l.c0 + c, 1.f));
             s1 += gm * (double)res[i * l.tx + k];
             s2 += gm * (double)res[(V + i) * l.tx + k];
         }
@@ -464,10 +484,11 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_backward_kerne
             const int r = l.row + u * l.ty;
             if (r < rows) {
                 float o[V];
+                const GnPack<T, V> xv = gn_fresh<4 + decltype(A)::value>(v[u]), dv = gn_fresh<4 + decltype(A)::value>(d[u]);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     float xhat, dz;
-                    ch.template value<decltype(A)::value>(i, gn_float(v[u].v[i]), gn_float(d[u].v[i]), xhat, dz);
+                    ch.template value<decltype(A)::value>(i, gn_float(xv.v[i]), gn_float(dv.v[i]), xhat, dz);
                     o[i] = ch.dx(i, xhat, dz, c1, c2);
                 }
                 gn_write<T, V>(dx + base + (int64_t)r * s.c, o);
@@ -527,7 +548,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_sums_kernel(const T* __restrict
                     a[1] = fma(d, d, a[1]);
                 }
             });
-        gn_sum_rows<double, 2>(a, l.tx, l.ty, l.row, res, lds);
+        gn_sum_rows<double, 2>(a, l.tx, l.ty, res, lds);
         // columns -> the groups that begin in or reach into this tile
         const int per = s.cg / V, k0 = tile * kGnThreads, k1 = k0 + l.tx, g0 = k0 / per;
         gn_each_group((k1 - 1) / per - g0 + 1, per, [&](int j, int lane, int lanes) {
@@ -633,8 +654,8 @@ __global__ __launch_bounds__(kGnThreads) void gn_grad_sums_kernel(const T* __res
                 });
             });
         }
-        gn_sum_rows<float, V>(a, l.tx, l.ty, l.row, res, lds);
-        gn_sum_rows<float, V>(b, l.tx, l.ty, l.row, res + V * l.tx, lds);
+        gn_sum_rows<float, V>(a, l.tx, l.ty, res, lds);
+        gn_sum_rows<float, V>(b, l.tx, l.ty, res + V * l.tx, lds);
         for (int c = threadIdx.x; c < l.tx * V; c += kGnThreads) {
             const int k = c / V, i = c - k * V;
             partial[((int64_t)n * s.chunks + chunk) * s.c + tile * kGnThreads * V + c] = make_float2(res[i * l.tx + k], res[(V + i) * l.tx + k]);
@@ -758,7 +779,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_backward_kernel(const T* __rest
 }
 
 // ------------------------------------------------------------------------------------------------ host
-static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype) {
+static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype, bool backward) {
     GnShape s;
     s.n = n; s.rows = rows; s.c = c; s.groups = groups; s.cg = c / groups;
     s.inv_m = 1.0 / ((double)rows * s.cg);
@@ -768,7 +789,10 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
     // resident, if all rows of a group fit (8 x 512 x 60 x 60 fp32 forward 28 us against 35 streamed, 1 x 256 x 64 x 64 9.5 against
     // 11.6, 8 x 512 x 20 x 20 6.3 against 11.6); more groups to a workgroup while its piece of a row is short of a cache line and there
     // are workgroups for every CU without.  Streamed for many rows of under 32 bytes, a fraction of each line that is fetched
-    // (8 x 256 x 90 x 90 fp32 in groups of 4 channels: 42 us resident, 38 streamed; 4 x 128 x 100 x 100 bf16: 19 against 16).
+    // (8 x 256 x 90 x 90 fp32 in groups of 4 channels: 42 us resident, 38 streamed; 4 x 128 x 100 x 100 bf16: 19 against 16).  The
+    // backward pass fetches twice as much, and streams where a workgroup has many rows (a whole line each, to one CU) and not every
+    // CU has a workgroup (2 x 256 x 64 x 64 fp32 25 us resident, 19 streamed; 3 x 90 x 61 x 47 fp16 18 against 13; 4 x 256 x 50 x 50 fp32
+    // 20 against 21, 8 x 256 x 64 x 64 bf16, 256 workgroups, 26 against 27).
     s.cs = s.threads = s.tx = s.ty = s.slabs = s.slab_groups = 0;
     s.tx_inverse = 0;
     const int held = gn_vectors_held(s.v, item);
@@ -780,14 +804,17 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
         int k = 1;
         for (int d = 2; d <= groups && (int64_t)k * s.cg * item < 128; ++d)
             if (groups % d == 0 && fits((int64_t)d * s.cg) && (int64_t)n * (groups / d) >= 256) k = d;
-        s.cs = k * s.cg;
+        const bool stream = backward && rows > 2600 && (int64_t)n * (groups / k) < 256;
+        s.cs = stream ? 0 : k * s.cg;
+    }
+    if (s.cs) {
         const int64_t tx = s.cs / s.v;
         // (two vectors a thread: enough loads in flight, and half the threads to add up)
         int64_t threads = (tx * ((rows + 1) / 2) + kWave - 1) / kWave * kWave;
         threads = threads > kGnResidentThreads ? kGnResidentThreads : threads;
         while (threads < tx || threads / tx * held < rows) threads += kWave;
         s.threads = (int32_t)threads;
-        s.tx = (int32_t)tx; s.ty = (int32_t)(threads / tx); s.slabs = groups / k; s.slab_groups = k;
+        s.tx = (int32_t)tx; s.ty = (int32_t)(threads / tx); s.slabs = c / s.cs; s.slab_groups = s.cs / s.cg;
         s.tx_inverse = (uint32_t)(((1 << 20) + tx - 1) / tx);
     }
     const int cv = c / s.v, ty = cv < kGnThreads ? kGnThreads / cv : 1, unroll = gn_rows_in_flight(s.v);
@@ -825,9 +852,13 @@ static GnWorkspace gn_workspace(void* base, const GnShape& s) {
 // dynamic LDS of the resident kernels: the groups' values, the columns' sums, and what gn_sum_rows works in
 static size_t gn_resident_lds(const GnShape& s, bool backward) {
     const int v = s.v;
-    const int64_t tx = s.cs / v, item = backward ? 4 : 8, width = backward ? v : 2;
-    const int64_t rows = tx <= kWave / 2 && (tx & (tx - 1)) == 0 ? (int64_t)s.threads / kWave * tx : s.threads;
-    return (size_t)(s.cs / s.cg * (backward ? 8 : 16) + ((backward ? 2 * v : 2) * tx + width * rows) * item);
+    const int64_t tx = s.cs / v, item = backward ? 4 : 8;
+    if (gn_whole_rows((int)tx)) {
+        const int64_t width = backward ? 2 * v : 2, weights = backward ? v : 0;
+        return (size_t)(s.cs / s.cg * (backward ? 8 : 16) + (width + weights + width * (s.threads / kWave)) * tx * item);
+    }
+    const int64_t width = backward ? (tx <= kGnResidentThreads / 2 ? 2 * v : v) : 2;
+    return (size_t)(s.cs / s.cg * (backward ? 8 : 16) + ((backward ? 2 * v : 2) * tx + width * s.threads) * item);
 }
 static int gn_check(const char* what, int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype, int wdtype, int act) {
     GEOMAE_REQUIRE(n >= 0 && rows >= 0 && c > 0 && groups > 0, "%s: bad shape [%d, %lld, %d] in %d groups", what, (int)n,
@@ -871,7 +902,7 @@ using namespace geomae;
 extern "C" int64_t geomae_group_norm_workspace_bytes(int32_t n, int64_t rows, int32_t c, int32_t groups, int32_t dtype, int32_t backward) {
     if (gn_check("group_norm_workspace_bytes", n, rows, c, groups, dtype, 0, 0)) return -1;
     if (n == 0 || rows == 0) return 0;
-    const GnShape s = gn_shape(n, rows, c, groups, dtype);
+    const GnShape s = gn_shape(n, rows, c, groups, dtype, backward != 0);
     if (gn_check_launches("group_norm_workspace_bytes", s)) return -1;
     const GnWorkspace w = gn_workspace(nullptr, s);
     return backward ? w.backward_bytes : w.forward_bytes;
@@ -884,7 +915,7 @@ extern "C" int geomae_group_norm_forward(const void* x, int32_t dtype, int32_t n
     GEOMAE_REQUIRE(eps >= 0.0, "group_norm_forward: eps must not be negative");
     if (n == 0 || rows == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(x && y && stats, "group_norm_forward: null argument");
-    const GnShape s = gn_shape(n, rows, c, groups, dtype);
+    const GnShape s = gn_shape(n, rows, c, groups, dtype, false);
     if (int rc = gn_check_launches("group_norm_forward", s)) return rc;
     const GnWorkspace ws = gn_workspace(workspace, s);
     if (workspace_bytes < ws.forward_bytes || (ws.forward_bytes && !workspace)) {
@@ -918,7 +949,7 @@ extern "C" int geomae_group_norm_backward(const void* x, const void* dy, int32_t
     if (int rc = gn_check("group_norm_backward", n, rows, c, groups, dtype, weight_dtype, activation)) return rc;
     if (n == 0 || rows == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(x && dy && stats && dx, "group_norm_backward: null argument");
-    const GnShape s = gn_shape(n, rows, c, groups, dtype);
+    const GnShape s = gn_shape(n, rows, c, groups, dtype, true);
     if (int rc = gn_check_launches("group_norm_backward", s)) return rc;
     const GnWorkspace ws = gn_workspace(workspace, s);
     if (workspace_bytes < ws.backward_bytes || (ws.backward_bytes && !workspace)) {
