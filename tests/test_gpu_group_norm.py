@@ -388,3 +388,22 @@ def test_capture_beside_a_graph_of_eager_work_is_refused(dev):
         graph.replay()
         want = torch.autograd.grad(ops.group_norm_act(x, 4, w, b), (w, b), dy)
         assert all(torch.equal(a, c) for a, c in zip(want, got))
+
+
+WORKGROUPS = [((1, 24, 40, 40), 1), ((2, 12, 30, 30), 1), ((2, 180, 9, 9), 1), ((2, 360, 9, 9), 1), ((2, 2056, 3), 1), ((1, 4096, 2), 1),
+              ((1, 4092, 2), 1), ((3, 20, 53, 50), 2), ((1, 20, 53, 50), 2), ((2, 64, 50, 52), 16), ((2, 64, 52, 51), 16), ((65, 6, 30), 2)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape,groups", WORKGROUPS, ids=[f"{'x'.join(map(str, s))}g{g}" for s, g in WORKGROUPS])
+def test_columns_and_rows_of_a_workgroup(dev, shape, groups, dtype):
+    """Columns that a wave does not hold whole rows of, few and many rows of them, more than half of the threads as columns, and
+    numbers of rows on both sides of the backward pass's choice of form; gamma negative and zero in places."""
+    x, dy, w, b = make(dev, shape, dtype, seed=5)
+    w[::3] *= -1
+    w[1::7] = 0
+    for act in ACTS:
+        want = reference(x, groups, w, b, 1e-5, act, dy)
+        got = run_both(x, groups, w, b, act, dy)
+        for k in want:
+            check(got[k], want[k], (act, k))
