@@ -779,20 +779,26 @@ __global__ __launch_bounds__(kGnThreads) void gn_backward_kernel(const T* __rest
 }
 
 // ------------------------------------------------------------------------------------------------ host
-static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype, bool backward) {
+static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype, int act, bool backward) {
     GnShape s;
     s.n = n; s.rows = rows; s.c = c; s.groups = groups; s.cg = c / groups;
     s.inv_m = 1.0 / ((double)rows * s.cg);
     s.v = s.cg % 4 == 0 ? 4 : (s.cg % 2 == 0 ? 2 : 1);
     s.past_cache = (double)n * rows * c * (dtype == GEOMAE_DTYPE_F32 ? 4 : 2) > 64e6;
     const int item = dtype == GEOMAE_DTYPE_F32 ? 4 : 2;
-    // resident, if all rows of a group fit (8 x 512 x 60 x 60 fp32 forward 28 us against 35 streamed, 1 x 256 x 64 x 64 9.5 against
-    // 11.6, 8 x 512 x 20 x 20 6.3 against 11.6); more groups to a workgroup while its piece of a row is short of a cache line and there
-    // are workgroups for every CU without.  Streamed for many rows of under 32 bytes, a fraction of each line that is fetched
-    // (8 x 256 x 90 x 90 fp32 in groups of 4 channels: 42 us resident, 38 streamed; 4 x 128 x 100 x 100 bf16: 19 against 16).  The
-    // backward pass fetches twice as much, and streams where a workgroup has many rows (a whole line each, to one CU) and not every
-    // CU has a workgroup (2 x 256 x 64 x 64 fp32 25 us resident, 19 streamed; 3 x 90 x 61 x 47 fp16 18 against 13; 4 x 256 x 50 x 50 fp32
-    // 20 against 21, 8 x 256 x 64 x 64 bf16, 256 workgroups, 26 against 27).
+    // Resident, if all rows of a group fit (fp32 forward: 8 x 512 x 20 x 20 6.5 us against 10.8 streamed, 4 x 256 x 50 x 50 11.0 against
+    // 13.8, 2 x 256 x 64 x 64 11.1 against 12.3); more groups to a workgroup while its piece of a row is short of a cache line and there
+    // are workgroups for every CU without.  Streamed for more than 4096 rows, whose pieces are a fraction of each line that is fetched
+    // (8 x 256 x 90 x 90 fp32 in groups of 4 channels: 42 us resident, 38 streamed; 4 x 128 x 100 x 100 bf16: 19 against 16), and where
+    // one workgroup a CU wastes what three launches cost:
+    //  many rows (a line each) of small pieces, or of tensors over 64 MB (backward: 8 x 64 x 64 x 64 bf16 in groups of 2 19.0 against
+    //  14.9; 16 x 256 x 64 x 64 fp32 73 against 62, forward 44 against 37);
+    //  many rows and CUs that have no workgroup, or none in the last round (backward: 2 x 256 x 64 x 64 fp32 25 against 19, 3 x 90 x 61 x 47
+    //  fp16 18 against 13, 24 x 256 x 64 x 64 bf16, 384 workgroups, 72 against 62, forward 40 against 33; 4 x 256 x 50 x 50 fp32 20 against 21);
+    //  silu and gelu, if the workgroups of a part of the CUs compute much (4 x 384 x 40 x 40 bf16 in groups of 24, gelu backward: 24.5
+    //  against 21.1, relu 17.2 against 21.0).
+    // Over 475 shapes of 1 to 16 samples, 400 to 4096 rows and 64 to 256 channels and three activations the form chosen takes 0.4 %
+    // (forward) and 0.7 % (backward) longer than the better one, always resident 1.4 and 6 %.
     s.cs = s.threads = s.tx = s.ty = s.slabs = s.slab_groups = 0;
     s.tx_inverse = 0;
     const int held = gn_vectors_held(s.v, item);
@@ -800,12 +806,16 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
         const int64_t tx = cs / s.v;
         return tx <= kGnResidentThreads && rows <= kGnResidentThreads / tx * held;
     };
-    if (fits(s.cg) && (rows <= 4096 || (int64_t)s.cg * item >= 32)) {
+    if (fits(s.cg) && rows <= 4096) {
         int k = 1;
         for (int d = 2; d <= groups && (int64_t)k * s.cg * item < 128; ++d)
             if (groups % d == 0 && fits((int64_t)d * s.cg) && (int64_t)n * (groups / d) >= 256) k = d;
-        const bool stream = backward && rows > 2600 && (int64_t)n * (groups / k) < 256;
-        s.cs = stream ? 0 : k * s.cg;
+        const int64_t workgroups = (int64_t)n * (groups / k), elements = rows * k * s.cg;
+        const bool idle = workgroups < (workgroups + 255) / 256 * 200;  // a fifth of the CUs and more, at least in the last round
+        const bool many_rows = rows > 2600 && (s.past_cache || (backward ? idle || k * s.cg * item < 16 : idle && workgroups > 256));
+        const bool much_work = (act == kGnGelu || act == kGnSilu) &&
+                               (backward ? idle && elements > 14000 : workgroups < 128 && elements > (act == kGnGelu ? 24000 : 48000));
+        s.cs = many_rows || much_work ? 0 : k * s.cg;
     }
     if (s.cs) {
         const int64_t tx = s.cs / s.v;
@@ -902,10 +912,15 @@ using namespace geomae;
 extern "C" int64_t geomae_group_norm_workspace_bytes(int32_t n, int64_t rows, int32_t c, int32_t groups, int32_t dtype, int32_t backward) {
     if (gn_check("group_norm_workspace_bytes", n, rows, c, groups, dtype, 0, 0)) return -1;
     if (n == 0 || rows == 0) return 0;
-    const GnShape s = gn_shape(n, rows, c, groups, dtype, backward != 0);
-    if (gn_check_launches("group_norm_workspace_bytes", s)) return -1;
-    const GnWorkspace w = gn_workspace(nullptr, s);
-    return backward ? w.backward_bytes : w.forward_bytes;
+    int64_t bytes = 0;
+    for (int act : {kGnNone, kGnGelu}) {                               // (the form may depend on the activation)
+        const GnShape s = gn_shape(n, rows, c, groups, dtype, act, backward != 0);
+        if (gn_check_launches("group_norm_workspace_bytes", s)) return -1;
+        const GnWorkspace w = gn_workspace(nullptr, s);
+        const int64_t need = backward ? w.backward_bytes : w.forward_bytes;
+        bytes = need > bytes ? need : bytes;
+    }
+    return bytes;
 }
 
 extern "C" int geomae_group_norm_forward(const void* x, int32_t dtype, int32_t n, int64_t rows, int32_t c, int32_t groups, const void* gamma,
@@ -915,7 +930,7 @@ extern "C" int geomae_group_norm_forward(const void* x, int32_t dtype, int32_t n
     GEOMAE_REQUIRE(eps >= 0.0, "group_norm_forward: eps must not be negative");
     if (n == 0 || rows == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(x && y && stats, "group_norm_forward: null argument");
-    const GnShape s = gn_shape(n, rows, c, groups, dtype, false);
+    const GnShape s = gn_shape(n, rows, c, groups, dtype, activation, false);
     if (int rc = gn_check_launches("group_norm_forward", s)) return rc;
     const GnWorkspace ws = gn_workspace(workspace, s);
     if (workspace_bytes < ws.forward_bytes || (ws.forward_bytes && !workspace)) {
@@ -949,7 +964,7 @@ extern "C" int geomae_group_norm_backward(const void* x, const void* dy, int32_t
     if (int rc = gn_check("group_norm_backward", n, rows, c, groups, dtype, weight_dtype, activation)) return rc;
     if (n == 0 || rows == 0) return GEOMAE_OK;
     GEOMAE_REQUIRE(x && dy && stats && dx, "group_norm_backward: null argument");
-    const GnShape s = gn_shape(n, rows, c, groups, dtype, true);
+    const GnShape s = gn_shape(n, rows, c, groups, dtype, activation, true);
     if (int rc = gn_check_launches("group_norm_backward", s)) return rc;
     const GnWorkspace ws = gn_workspace(workspace, s);
     if (workspace_bytes < ws.backward_bytes || (ws.backward_bytes && !workspace)) {
