@@ -20,7 +20,8 @@
 // What bounds it: HBM.  Bytes per element: fp32 parameters 28 with 32-bit moments (p, m, v in and out, g in) and 16 1/8 with
 // 8-bit ones.  A workgroup takes a chunk of 4096 elements of one tensor, found through a table built once; the gradients'
 // addresses, which change from step to step, ride in the launch's arguments, so that no copy to the device and no state of the
-// call's own stands between two steps or inside a captured graph.
+// call's own stands between two steps or inside a captured graph.  Measured: 40 M fp32 elements, 32-bit moments 214 us (1.12 GB, 5.2
+// TB/s); 48 M bf16 elements with masters, 8-bit moments 140 us (0.77 GB, 5.5 TB/s) and 33 us for the norm before it (96 MB, 2.9 TB/s).
 #include "common.h"
 #include "../../include/geomae_hip.h"
 #include <math.h>
@@ -422,6 +423,7 @@ __global__ __launch_bounds__(kMaThreads) void multi_adamw_kernel(MaStepArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ codes -> values
+// HBM: 2 1/16 bytes in and 4 out per element; 48 M elements 61 us (291 MB, 4.8 TB/s).
 __global__ __launch_bounds__(256) void adamw_moments8_kernel(const uint32_t* m, const uint8_t* me, const uint32_t* r, const uint8_t* re,
                                                             int64_t words, uint2* m_out, uint2* r_out) {
     auto put = [](uint2* out, int64_t i, const float (&x)[kMaVec]) {
