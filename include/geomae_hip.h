@@ -820,7 +820,7 @@ int geomae_adamw_moments8(const uint8_t* exp_avg, const uint8_t* exp_avg_exponen
 
 /* ------------------------------------------------------------------ group norm with an activation, channels last
  * x, y, dy, dx: [n][rows][c] of `dtype` (GEOMAE_DTYPE_*); a group is c / groups neighbouring channels of a sample (at most
- * 1024 groups).  y = act(gamma (x - mean) / sqrt(var + eps) + beta), var biased; gamma, beta [c] of weight_dtype, or NULL (1, 0).
+ * 1024 groups and 2^22 channels).  y = act(gamma (x - mean) / sqrt(var + eps) + beta), var biased; gamma, beta [c] of weight_dtype, or NULL (1, 0).
  * stats [n][groups][2] fp64 (16-byte aligned) receives (mean, 1 / sqrt(var + eps)): the backward pass reads it.  dgamma, dbeta [c] of
  * weight_dtype, or NULL.  ReLU's derivative at 0 is 0; gelu is the erf form.  workspace: the forward and the backward pass need
  * geomae_group_norm_workspace_bytes(..., backward = 0 / 1) bytes each (-1: bad shape), 16-byte aligned. */

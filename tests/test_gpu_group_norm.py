@@ -392,7 +392,7 @@ def test_capture_beside_a_graph_of_eager_work_is_refused(dev):
 
 WORKGROUPS = [((1, 24, 40, 40), 1), ((2, 12, 30, 30), 1), ((2, 180, 9, 9), 1), ((2, 360, 9, 9), 1), ((2, 2056, 3), 1), ((1, 4096, 2), 1),
               ((1, 4092, 2), 1), ((3, 20, 53, 50), 2), ((1, 20, 53, 50), 2), ((2, 64, 50, 52), 16), ((2, 64, 52, 51), 16), ((65, 6, 30), 2),
-              ((1, 64, 40, 40), 1), ((2, 32, 28, 28), 1), ((10, 64, 52, 52), 32)]
+              ((1, 64, 40, 40), 1), ((2, 32, 28, 28), 1), ((10, 64, 52, 52), 32), ((1, 1 << 20, 5), 1024), ((1, (1 << 20) + 1, 3), 1)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])

@@ -88,3 +88,10 @@ def test_more_threads_than_a_launch_counts_are_refused():
     assert lib.geomae_group_norm_workspace_bytes(1 << 26, 1, 64, 8, 1, 0) == -1 and b"too many" in lib.geomae_last_error()
     assert lib.geomae_group_norm_forward(64, 1, 1 << 26, 1, 64, 8, None, None, 0, 1e-5, 0, 64, 64, None, 0, None) < 0
     assert lib.geomae_group_norm_backward(64, 64, 1, 1 << 26, 1, 64, 8, None, None, 0, 0, 64, 64, None, None, None, 0, None) < 0
+
+
+def test_channels_that_32_bit_offsets_do_not_reach_are_refused():
+    from geomae_amd import _lib
+    lib = _lib.load()
+    assert lib.geomae_group_norm_workspace_bytes(1, 5, 1 << 22, 1024, 0, 0) >= 0
+    assert lib.geomae_group_norm_workspace_bytes(1, 5, (1 << 22) + 1024, 1024, 0, 0) == -1 and b"channels" in lib.geomae_last_error()
