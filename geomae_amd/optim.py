@@ -194,7 +194,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------------------------------------ the step
     def step(self, closure=None, max_norm=0.0, grad_scale=1.0, skip_nonfinite=False):
         """One update of every parameter that has a gradient.  max_norm > 0 clips the gradients to that norm over all of
-        them (torch.nn.utils.clip_grad_norm_; infinity: only the norm is wanted); grad_scale (a number, or one float32 value on the GPU) multiplies them first;
+        them (torch.nn.utils.clip_grad_norm_; infinity: only the norm is wanted; 0 or None: no clipping); grad_scale (a number, or one
+        float32 value on the GPU) multiplies them first;
         skip_nonfinite leaves everything as it was if their norm is not finite.  After a step with max_norm or
         skip_nonfinite, `grad_norm` is the scaled gradients' norm before clipping (a 0-d tensor that the next step
         overwrites).  Gradients are not changed."""
