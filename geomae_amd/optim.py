@@ -29,6 +29,13 @@ def _dense(t):
     return True
 
 
+def _memory_order(t):
+    """The dimensions of a dense tensor from the slowest in memory to the fastest, without those of one element."""
+    if t.numel() == 0:
+        return []
+    return [d for _, d in sorted(((-t.stride(d), d) for d in range(t.dim()) if t.shape[d] != 1))]
+
+
 class MultiTensorAdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update (decoupled weight decay) of all parameters in two launches per 384 tensors, whatever their sizes.
 
@@ -288,12 +295,16 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     def state_dict(self):
         sd = super().state_dict()
         sd["state_bits"], sd["master_weights"], sd["seed"] = self.state_bits, self.master_weights, self.seed
+        if self.state_bits == 8:
+            # an exponent byte belongs to 32 codes in memory order, whatever order a saved tensor of codes has by the time it is loaded
+            sd["memory_orders"] = [_memory_order(p) for p in self._params()]
         return sd
 
     @torch.no_grad()
     def load_state_dict(self, sd):
         """A state_dict of this class with the same state_bits and masters, or (32 bits) one of torch.optim.AdamW.  Parameters
-        that it has no state of begin anew; masters that it does not hold are taken from the parameters."""
+        that it has no state of begin anew; masters that it does not hold are taken from the parameters.  An 8-bit state of a parameter
+        in another memory order (contiguous, now channels_last) is refused: its blocks are other elements here."""
         if int(sd.get("state_bits", 32)) != self.state_bits:
             raise ValueError(f"the state holds moments in {sd.get('state_bits', 32)} bits, this optimizer in {self.state_bits}")
         groups = sd["param_groups"]
@@ -302,9 +313,17 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if any(g.get("amsgrad") or g.get("maximize") for g in groups):
             raise ValueError("amsgrad and maximize are not supported")
         params, ids = self._params(), [i for g in groups for i in g["params"]]
-        todo = []
-        for p, i in zip(params, ids):
+        todo, orders = [], sd.get("memory_orders")
+        if orders is not None and len(orders) != len(params):
+            raise ValueError(f"the state has memory orders of {len(orders)} parameters, this optimizer has {len(params)}")
+        for n, (p, i) in enumerate(zip(params, ids)):
             st, mine = sd["state"].get(i), self.state[p]
+            if st is not None and self.state_bits == 8 and "exp_avg" in st and "exp_avg_sq" in st:
+                for k in ("exp_avg", "exp_avg_sq"):
+                    order = _memory_order(st[k]) if orders is None else list(orders[n])
+                    if order != _memory_order(p):
+                        raise ValueError(f"the state of parameter {i}: {k} has codes with the dimensions in memory order {order}, the "
+                                         f"parameter {_memory_order(p)}; their exponents are of 32 neighbours in memory")
             if st is None:
                 st = {k: torch.full((), _ZERO_EXPONENT if k.endswith("exponent") else 0, dtype=v.dtype).expand(v.shape)
                       for k, v in mine.items() if k != "master"}

@@ -561,3 +561,38 @@ def test_hooks_profiler_and_subclasses(dev):
             opt.step()
         assert sum(f"Optimizer.step#{cls.__name__}.step" in e.name for e in prof.events()) == 1
         assert int(opt.state[p]["step"]) == 4 and getattr(opt, "count", 4) == 4
+
+
+def test_codes_stay_with_their_exponents_in_another_memory_order(dev):
+    """An 8-bit state is refused by a parameter of the same shape in another memory order (32 elements that share an exponent are
+    others there) and leaves the optimizer as it was; in its own order it is the same whatever the saved tensors' strides are;
+    32 bits go across."""
+    gen = torch.Generator().manual_seed(1)
+    base = torch.randn(64, 16, 3, 3, generator=gen) * torch.exp(2 * torch.randn(64, 16, 3, 3, generator=gen))
+    lin = torch.randn(24, 40, generator=gen)
+    kinds = {"rows": (base, lin), "columns": (base.to(memory_format=torch.channels_last), lin.t().contiguous().t())}
+
+    def stepped(kind, bits):
+        params = [torch.nn.Parameter(t.to(dev, copy=True)) for t in kinds[kind]]
+        for p in params:
+            p.grad = torch.sin(1e3 * p.detach()) * p.detach().abs()
+        opt = new(params, state_bits=bits, seed=4)
+        opt.step()
+        return opt, params
+    for src, dst in (("rows", "columns"), ("columns", "rows"), ("rows", "rows"), ("columns", "columns")):
+        for bits in (8, 32):
+            a, ps = stepped(src, bits)
+            sd = a.state_dict()
+            flat = {**sd, "state": {i: {k: v.contiguous() for k, v in st.items()} for i, st in sd["state"].items()}}
+            old = {k: v for k, v in sd.items() if k != "memory_orders"}                    # (as it was written before)
+            for state in (sd, flat, old):
+                b, qs = stepped(dst, bits)
+                held = [t.clone() for t in b._arena.values()]
+                if bits == 8 and src != dst:
+                    with pytest.raises(ValueError, match="memory order"):
+                        b.load_state_dict(state)
+                    assert all(torch.equal(x, y) for x, y in zip(held, b._arena.values()))
+                    continue
+                b.load_state_dict(state)
+                for p, q in zip(ps, qs):
+                    assert all(torch.equal(a.state[p][k], b.state[q][k]) for k in a.state[p])

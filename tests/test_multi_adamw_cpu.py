@@ -127,3 +127,12 @@ def test_a_clipping_norm_is_not_negative():
     for bad in (-1.0, float("nan")):
         assert lib.geomae_multi_adamw_step(64, 64, one, 1, grads, which, ctypes.addressof(hypers), 1, 32, bad, 1.0, None, 0, 0, None, None,
                                            0, None) < 0 and b"max_norm" in lib.geomae_last_error()
+
+
+def test_memory_orders():
+    from geomae_amd.optim import _memory_order
+    x = torch.empty(2, 3, 4, 5)
+    assert _memory_order(x) == [0, 1, 2, 3] and _memory_order(x.to(memory_format=torch.channels_last)) == [0, 2, 3, 1]
+    assert _memory_order(torch.empty(3, 4).t()) == [1, 0] and _memory_order(torch.empty(())) == [] == _memory_order(torch.empty(0, 4))
+    one = torch.empty(6, 1, 5, 1)                                         # dimensions of one element do not count
+    assert _memory_order(one) == [0, 2] == _memory_order(one.to(memory_format=torch.channels_last))
