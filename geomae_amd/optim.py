@@ -59,7 +59,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         self.state_bits, self.master_weights, self.seed = int(state_bits), bool(master_weights), int(seed)
         if not 0 <= self.seed < 2 ** 32:
             raise ValueError("seed must be in [0, 2**32)")
-        self._arena, self._table, self._building, self._plan, self._retired = None, None, True, None, []
+        self._arena, self._building, self._plan, self._layout, self._retired = None, True, None, [], []
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         self._building = False
@@ -75,6 +75,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise ValueError(f"lr, eps and weight_decay must not be negative, got {g['lr']}, {g['eps']}, {g['weight_decay']}")
 
     def add_param_group(self, group):
+        """A refused group leaves the optimizer as it was.  A step that was captured before goes on with the state of that time:
+        capture it anew."""
         super().add_param_group(group)
         g = self.param_groups[-1]
         try:
@@ -83,11 +85,11 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                 raise ValueError("a tensor lr must be one float32 value on the GPU")
             self._check_params(g["params"])
             self._check_apart()
+            if not self._building:
+                self._build()
         except Exception:
             self.param_groups.pop()
             raise
-        if not self._building:
-            self._build()
 
     def _check_params(self, params):
         first = self.param_groups[0]["params"][0]
@@ -113,9 +115,12 @@ class MultiTensorAdamW(torch.optim.Optimizer):
 
     def _build(self):
         """Moments of all parameters in one arena per kind, each parameter's part starting at a multiple of 32 elements; a
-        parameter's state tensors are views of it in the parameter's own layout.  Parameters that were there keep theirs."""
-        self._retire()
-        params, old = self._params(), self._arena
+        parameter's state tensors are views of it in the parameter's own layout.  Parameters that were there keep theirs.  Nothing
+        of the optimizer changes before all of it is there."""
+        params, had = self._params(), len(self._layout)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("MultiTensorAdamW: parameters cannot be added while a stream is captured")
+        self._check_layout(params[:had])
         dev = params[0].device
         offsets, total = [], 0
         for p in params:
@@ -129,16 +134,13 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                 arena[k] = torch.full((total // BLOCK,), _ZERO_EXPONENT, dtype=torch.uint8, device=dev)
         if self.master_weights:
             arena["master"] = torch.zeros(total, dtype=torch.float32, device=dev)
-        self._arena, self.offsets = arena, offsets
-        for i, (p, off) in enumerate(zip(params, offsets)):
-            had = self.state.get(p) if old is not None else None
-            new = self._views(arena, i, p, off)
+        state = [self._views(arena, i, p, off) for i, (p, off) in enumerate(zip(params, offsets))]
+        for i, (p, new) in enumerate(zip(params, state)):
             for k, v in new.items():
-                if had:
-                    v.copy_(had[k])
+                if i < had:
+                    v.copy_(self.state[p][k])
                 elif k == "master":
                     v.copy_(p.detach())
-            self.state[p] = new
         lib = _lib.load()
         chunk = lib.geomae_multi_adamw_chunk()
         counts = [-(-p.numel() // chunk) for p in params]
@@ -147,13 +149,11 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             first.append(first[-1] + c)
         tensor = torch.repeat_interleave(torch.arange(len(params), dtype=torch.int32), torch.tensor(counts, dtype=torch.int64))
         within = torch.arange(first[-1], dtype=torch.int64) - torch.tensor(first[:-1], dtype=torch.int64)[tensor.long()]
-        self._chunks = torch.stack([tensor, within.int()], 1).contiguous().to(dev)
-        n = len(params)
-        self._first_chunk = first
-        ws = lib.geomae_multi_adamw_workspace_bytes(n)
-        self._workspace = torch.empty(ws, dtype=torch.uint8, device=dev)
-        self._norm_word = torch.zeros((), dtype=torch.float32, device=dev)
-        self._fill_table()
+        chunks = torch.stack([tensor, within.int()], 1).contiguous().to(dev)
+        workspace = torch.empty(lib.geomae_multi_adamw_workspace_bytes(len(params)), dtype=torch.uint8, device=dev)
+        norm_word = torch.zeros((), dtype=torch.float32, device=dev)
+        self._set_table(params, arena, offsets, chunks, first, workspace, norm_word)
+        self.state.update(zip(params, state))
 
     def _retire(self):
         """What a captured step may still read and write is kept as long as this optimizer."""
@@ -176,27 +176,35 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             out["master"] = self._part(arena["master"], off, p)
         return out
 
-    def _fill_table(self):
-        """The device table of addresses."""
-        params, a = self._params(), self._arena
+    def _set_table(self, params, arena, offsets, chunks, first_chunk, workspace, norm_word):
+        """Take these buffers, with a device table of the addresses in them."""
         rows = (_lib.GeomaeAdamwTensor * len(params))()
-        for i, (p, off) in enumerate(zip(params, self.offsets)):
+        item = arena["exp_avg"].element_size()
+        for i, (p, off) in enumerate(zip(params, offsets)):
             r = rows[i]
-            item = a["exp_avg"].element_size()
             r.param = p.data_ptr()
-            r.exp_avg, r.exp_avg_sq = a["exp_avg"].data_ptr() + off * item, a["exp_avg_sq"].data_ptr() + off * item
+            r.exp_avg, r.exp_avg_sq = arena["exp_avg"].data_ptr() + off * item, arena["exp_avg_sq"].data_ptr() + off * item
             if self.state_bits == 8:
-                r.exp_avg_exponent = a["exp_avg_exponent"].data_ptr() + off // BLOCK
-                r.exp_avg_sq_exponent = a["exp_avg_sq_exponent"].data_ptr() + off // BLOCK
-            r.master = a["master"].data_ptr() + 4 * off if self.master_weights and p.dtype != torch.float32 else None
-            r.step = a["step"].data_ptr() + 8 * i
+                r.exp_avg_exponent = arena["exp_avg_exponent"].data_ptr() + off // BLOCK
+                r.exp_avg_sq_exponent = arena["exp_avg_sq_exponent"].data_ptr() + off // BLOCK
+            r.master = arena["master"].data_ptr() + 4 * off if self.master_weights and p.dtype != torch.float32 else None
+            r.step = arena["step"].data_ptr() + 8 * i
             r.numel, r.dtype, r.index = p.numel(), _DTYPE[p.dtype], i
-        host = torch.frombuffer(bytearray(rows), dtype=torch.uint8)
+        table = torch.frombuffer(bytearray(rows), dtype=torch.uint8).to(params[0].device)
+        plan = _lib.host().AdamwPlan(params, first_chunk, table.data_ptr(), chunks.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                                     norm_word.data_ptr(), self.state_bits)
         self._retire()
-        self._table = host.to(params[0].device)
-        self._layout = [(p.shape, p.stride(), p.dtype, p.device) for p in params]
-        self._plan = _lib.host().AdamwPlan(params, self._first_chunk, self._table.data_ptr(), self._chunks.data_ptr(),
-                                           self._workspace.data_ptr(), self._workspace.numel(), self._norm_word.data_ptr(), self.state_bits)
+        self._arena, self.offsets, self._chunks, self._first_chunk = arena, offsets, chunks, first_chunk
+        self._workspace, self._norm_word, self._table, self._plan = workspace, norm_word, table, plan
+        self._layout = self._layouts(params)
+
+    @staticmethod
+    def _layouts(params):
+        return [(p.shape, p.stride(), p.dtype, p.device) for p in params]
+
+    def _check_layout(self, params):
+        if self._layouts(params) != self._layout:
+            raise RuntimeError("MultiTensorAdamW: a parameter changed its shape, layout, dtype or device; make a new optimizer")
 
     # ------------------------------------------------------------------------------------------------ the step
     def step(self, closure=None, max_norm=0.0, grad_scale=1.0, skip_nonfinite=False):
@@ -240,13 +248,12 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     def _find_params(self):
         """A parameter is not where or what the device table says: make the table anew."""
         params = self._params()
-        if [(p.shape, p.stride(), p.dtype, p.device) for p in params] != self._layout:
-            raise RuntimeError("MultiTensorAdamW: a parameter changed its shape, layout, dtype or device; make a new optimizer")
+        self._check_layout(params)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("MultiTensorAdamW: a parameter's storage moved; take one step outside the capture first")
         self._check_params(params)
         self._check_apart()
-        self._fill_table()
+        self._set_table(params, self._arena, self.offsets, self._chunks, self._first_chunk, self._workspace, self._norm_word)
 
     # ------------------------------------------------------------------------------------------------ state
     def moments(self):

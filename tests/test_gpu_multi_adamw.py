@@ -596,3 +596,29 @@ def test_codes_stay_with_their_exponents_in_another_memory_order(dev):
                 b.load_state_dict(state)
                 for p, q in zip(ps, qs):
                     assert all(torch.equal(a.state[p][k], b.state[q][k]) for k in a.state[p])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_group_is_refused_beside_a_changed_parameter(dev, bits):
+    """A parameter that was cut, cast or re-ordered in the meantime: the new group is refused, and with the parameter as it was the
+    optimizer goes on as if nothing had been asked of it."""
+    changes = (lambda t: t[:3], lambda t: t.half(), lambda t: t.contiguous(memory_format=torch.channels_last), lambda t: t.transpose(0, 1))
+    for change in changes:
+        params = [torch.nn.Parameter(torch.randn(s, generator=torch.Generator().manual_seed(7)).bfloat16().to(dev)) for s in ((8, 6, 5, 3), (70,))]
+        twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+        for p, q in zip(params, twins):
+            p.grad = torch.randn_like(p)
+            q.grad = p.grad
+        a, b = (new(s, state_bits=bits, master_weights=True) for s in (params, twins))
+        a.step()
+        b.step()
+        grad, kept = params[0].grad, params[0].data
+        params[0].grad, params[0].data = None, change(kept)
+        with pytest.raises(RuntimeError, match="shape, layout"):
+            a.add_param_group({"params": [torch.nn.Parameter(torch.zeros(9, device=dev))]})
+        assert len(a.param_groups) == 1 and len(a.state) == 2
+        params[0].data, params[0].grad = kept, grad
+        a.step(max_norm=1.0)
+        b.step(max_norm=1.0)
+        assert all(torch.equal(p, q) for p, q in zip(params, twins))
+        assert all(torch.equal(a.state[p][k], v) for p, q in zip(params, twins) for k, v in b.state[q].items())
