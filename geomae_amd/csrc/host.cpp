@@ -4,6 +4,7 @@
 // C ABI of libgeomae_hip, whose entry points bind() takes by address.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include "../../include/geomae_hip.h"
@@ -295,6 +296,10 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 at::Tensor group_norm_act(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight_, const c10::optional<at::Tensor>& bias_,
                           double eps, const c10::optional<std::string>& activation) {
     const at::Tensor weight = weight_.value_or(at::Tensor()), bias = bias_.value_or(at::Tensor());
+    // (a kernel that neither sees would give a zero derivative, and a trace that returns memory nobody wrote)
+    for (const at::Tensor& t : {x, weight, bias})
+        TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "group_norm_act has no forward-mode derivative");
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), "group_norm_act cannot be traced by torch.jit.trace");
     TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (geomae_amd has no CPU path)");
     TORCH_CHECK(x.dim() >= 2, "x must be [N, C, *], got ", x.sizes());
     TORCH_CHECK(dtype_code(x.scalar_type()) >= 0, "x must be float32, bfloat16 or float16, got ", x.scalar_type());

@@ -95,3 +95,21 @@ def test_channels_that_32_bit_offsets_do_not_reach_are_refused():
     lib = _lib.load()
     assert lib.geomae_group_norm_workspace_bytes(1, 5, 1 << 22, 1024, 0, 0) >= 0
     assert lib.geomae_group_norm_workspace_bytes(1, 5, (1 << 22) + 1024, 1024, 0, 0) == -1 and b"channels" in lib.geomae_last_error()
+
+
+def test_forward_mode_and_traces_are_refused():
+    """A dual tensor does not require a gradient, and a trace records no kernel: both would come back without an error as a zero
+    derivative and as memory that nothing wrote."""
+    import torch.autograd.forward_ad as fwAD
+    from geomae_amd import ops
+    x, w, b = torch.randn(2, 4), torch.ones(4), torch.zeros(4)
+    for grad in (torch.enable_grad, torch.no_grad):
+        with grad(), fwAD.dual_level():
+            for k in range(3):
+                args = [fwAD.make_dual(t, torch.ones_like(t)) if i == k else t for i, t in enumerate((x, w, b))]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    ops.group_norm_act(args[0], 2, args[1], args[2])
+        with grad(), pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(lambda t: ops.group_norm_act(t, 2), (x,), check_trace=False)
+    with pytest.raises(RuntimeError, match="CUDA"):                       # (outside of both it is the device that is refused)
+        ops.group_norm_act(x, 2, w, b)
