@@ -491,10 +491,10 @@ __device__ __forceinline__ float gelu_f(float x) {
     gelu_parts(x, &c, &p);
     return x * c;
 }
-// The same on the four values of an accumulator register group, two at a time on the packed fp32 pipe (v_pk_mul_f32 /
-// v_pk_fma_f32 process two floats per lane and issue slot): 17 full-rate + 4 quarter-rate instructions per PAIR instead
-// of 14 + 2 per value.  The GELU arithmetic is VALU-bound: 64 evaluations per lane and kernel were 7.2 k of the 46 k
-// cycles of a workgroup in sst_ffn_bwd_kernel (tools/archive/phase_timing.py).
+// The same on the four values of an accumulator register group, in pairs: 14 full-rate + 2 quarter-rate instructions per value
+// (packed fp32 arithmetic, which would halve the first, is off: build.py).  64 evaluations per lane and kernel are about a seventh of
+// the cycles of a workgroup in sst_ffn_bwd_kernel (tools/archive/phase_timing.py); without the packed instructions the step is the same
+// to half a percent, as the kernels wait more than they issue.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void gelu_parts2(f32x2 x, f32x2* cdf, f32x2* pdf) {
     const f32x2 ax = {__builtin_fabsf(x.x), __builtin_fabsf(x.y)};

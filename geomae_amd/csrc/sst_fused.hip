@@ -502,7 +502,7 @@ __device__ __forceinline__ void fused_bwd_body(const FusedBwd& A, const int s0, 
     uint4 w2a[4], w2b[4];
     load_wfrag<128>(W.frag + kOffW2T, 2 * w, lane, w2a);
     load_wfrag<128>(W.frag + kOffW2T, 2 * w + 1, lane, w2b);
-    const f32x4 g2 = load_f4(W.g2 + 16 * w + 4 * g), g1 = load_f4(W.g1 + 16 * w + 4 * g);
+    const f32x4 g2 = load_f4(W.g2 + 16 * w + 4 * g);
 
     // ---- LayerNorm-2 backward: d <- rstd2 (d g2 - mean(d g2) - xhat2 mean(d g2 xhat2)); parameter gradients of this tile
     f32x4 pg = {0.f, 0.f, 0.f, 0.f}, pb = {0.f, 0.f, 0.f, 0.f};       // sum_t d * xhat, sum_t d (this lane's token column)
@@ -588,6 +588,8 @@ __device__ __forceinline__ void fused_bwd_body(const FusedBwd& A, const int s0, 
     FUSED_STAMP(6);
 
     // ---- dy = d(y + f) + dhp W1 (channel tile w); LayerNorm-1 backward
+    // (its gamma is fetched here, in flight under the GEMM: across the FFN backward its four registers made the NT = 4 body spill two)
+    const f32x4 g1 = load_f4(W.g1 + 16 * w + 4 * g);
     pg = f32x4{0.f, 0.f, 0.f, 0.f}; pb = pg;
     FOR_TILES(it) {
         const char* row = RH + (16 * it + t) * kFRowH + 16 * g;

@@ -56,3 +56,17 @@ def test_hot_layer_kernels_stay_inside_their_register_budget():
             seen.append((name, v))
             assert v["scratch"] <= max_scratch and v["spill"] <= max_spill and v["lds"] <= max_lds and v["vgpr"] <= 256, (name, v)
     print(seen)
+
+
+def test_no_source_is_built_with_packed_fp32():
+    """Every kernel source, without an exception, and no inline assembly either."""
+    import sys
+    sys.path.insert(0, ROOT)
+    from geomae_amd.csrc import build
+    assert len(build.sources()) > 15
+    for src in build.sources():
+        flags = " ".join(build.flags_for(src))
+        assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in flags, src
+    for name in os.listdir(SRC):
+        if name.endswith((".hip", ".h")):
+            assert not re.search(r"v_pk_(add|mul|fma)_f32", open(os.path.join(SRC, name)).read()), name
