@@ -341,21 +341,31 @@ class FlatAdamW:
                                weight_decay=wd, amsgrad=False))
         return dict(state=state, param_groups=groups)
 
-    def load_state_dict(self, sd):
+    def check_state(self, sd):
+        """ValueError if load_state_dict() would refuse this state."""
+        if int(sd.get("state_bits", 32)) != 32:
+            raise ValueError(f"the optimizer state holds moments in {sd['state_bits']} bits, this optimizer in 32")
         order = self._checkpoint_order()
         extra = [k for k in sd["state"] if not (isinstance(k, int) and 0 <= k < len(order))]
         if extra:
             raise ValueError(f"optimizer state has entries for parameters this model does not have: {extra[:4]}")
         for i, (p, off) in enumerate(order):
+            st = sd["state"].get(i)
+            if st is None or off is None:
+                continue
+            for key in ("exp_avg", "exp_avg_sq"):
+                if tuple(st[key].shape) != tuple(p.shape):
+                    raise ValueError(f"optimizer state {i}: {key} has shape {tuple(st[key].shape)}, the parameter "
+                                     f"{tuple(p.shape)} (the checkpoint is from a different model or parameter order)")
+                if not st[key].is_floating_point():
+                    raise ValueError(f"optimizer state {i}: {key} is {st[key].dtype}, not the moment's values")
+
+    def load_state_dict(self, sd):
+        self.check_state(sd)                         # (all of it first: a refused state changes nothing)
+        for i, (p, off) in enumerate(self._checkpoint_order()):
             n = p.numel()
             st = sd["state"].get(i)
-            if st is not None and off is None:
-                continue                         # state of a parameter that is frozen here: nothing to restore
-            if st is not None:
-                for key in ("exp_avg", "exp_avg_sq"):
-                    if tuple(st[key].shape) != tuple(p.shape):
-                        raise ValueError(f"optimizer state {i}: {key} has shape {tuple(st[key].shape)}, the parameter "
-                                         f"{tuple(p.shape)} (the checkpoint is from a different model or parameter order)")
+            if st is not None and off is not None:   # (state of a parameter that is frozen here: nothing to restore)
                 self.exp_avg[off:off + n].copy_(st["exp_avg"].reshape(-1))
                 self.exp_avg_sq[off:off + n].copy_(st["exp_avg_sq"].reshape(-1))
                 self.step_count = int(float(st["step"]))

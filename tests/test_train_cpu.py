@@ -309,3 +309,28 @@ def test_checkpoint_indices_count_frozen_parameters(tmp_path):
     l1, _ = tr.train_step(x)
     l2, _ = tr2.train_step(x)
     assert torch.equal(l1["loss"], l2["loss"])
+
+
+def test_flat_adamw_refuses_codes_and_a_refused_state_changes_nothing():
+    """8-bit codes (optim.MultiTensorAdamW) of the parameters' shapes are not moments; a state whose last entry does not fit leaves the
+    first ones alone."""
+    torch.manual_seed(0)
+    flat = FlatParams(Toy(), no_decay_keys=("norm",))
+    opt = FlatAdamW(flat)
+    opt.exp_avg.normal_()
+    opt.exp_avg_sq.uniform_()
+    good = opt.state_dict()
+    kept = opt.exp_avg.clone(), opt.exp_avg_sq.clone()
+    codes = {i: dict(step=torch.tensor(3), exp_avg=torch.full_like(st["exp_avg"], 56, dtype=torch.uint8),
+                     exp_avg_sq=torch.full_like(st["exp_avg_sq"], 99, dtype=torch.uint8)) for i, st in good["state"].items()}
+    other = {i: dict(step=torch.tensor(3.0), exp_avg=torch.ones_like(st["exp_avg"]), exp_avg_sq=torch.ones_like(st["exp_avg_sq"]))
+             for i, st in good["state"].items()}
+    last = max(other)
+    short = {**other, last: {**other[last], "exp_avg_sq": torch.ones(1)}}
+    for sd, match in ((dict(good, state=codes), "uint8"), (dict(good, state=other, state_bits=8), "8 bits"), (dict(good, state=short), "shape"),
+                      (dict(good, state={**other, 99: other[0]}), "does not have")):
+        with pytest.raises(ValueError, match=match):
+            opt.load_state_dict(sd)
+        assert torch.equal(opt.exp_avg, kept[0]) and torch.equal(opt.exp_avg_sq, kept[1]) and opt.step_count == 0
+    opt.load_state_dict(dict(good, state=other))
+    assert opt.step_count == 3 and all((opt.exp_avg[o:o + p.numel()] == 1).all() for p, o in zip(flat.params, flat.offsets))
