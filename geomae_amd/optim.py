@@ -277,6 +277,10 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise RuntimeError("MultiTensorAdamW: made without master_weights")
         return self._arena["master"]
 
+    def steps(self):
+        """The steps that each parameter has taken, as an int64 tensor (not a copy)."""
+        return self._arena["step"]
+
     @torch.no_grad()
     def sync_masters(self):
         """Take the masters from the parameters."""
@@ -307,11 +311,14 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             sd["memory_orders"] = [_memory_order(p) for p in self._params()]
         return sd
 
-    @torch.no_grad()
     def load_state_dict(self, sd):
         """A state_dict of this class with the same state_bits and masters, or (32 bits) one of torch.optim.AdamW.  Parameters
         that it has no state of begin anew; masters that it does not hold are taken from the parameters.  An 8-bit state of a parameter
         in another memory order (contiguous, now channels_last) is refused: its blocks are other elements here."""
+        self.check_state(sd)()
+
+    def check_state(self, sd):
+        """ValueError if load_state_dict() would refuse this state; else the function that takes it."""
         if int(sd.get("state_bits", 32)) != self.state_bits:
             raise ValueError(f"the state holds moments in {sd.get('state_bits', 32)} bits, this optimizer in {self.state_bits}")
         groups = sd["param_groups"]
@@ -346,10 +353,14 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                 todo.append((v, x.reshape(v.shape)))
         for g, h in zip(self.param_groups, groups):
             self._check_hyper({**g, **{k: v for k, v in h.items() if k != "params"}})
-        for v, x in todo:
-            v.copy_(x)
-        for g, h in zip(self.param_groups, groups):
-            mine, lr = g["lr"], float(h.get("lr", g["lr"]))
-            g.update({k: v for k, v in h.items() if k != "params"})
-            g["lr"] = mine.fill_(lr) if torch.is_tensor(mine) else lr   # (a captured step reads a tensor lr where it is)
-        self.seed = int(sd.get("seed", self.seed))
+
+        @torch.no_grad()
+        def take():
+            for v, x in todo:
+                v.copy_(x)
+            for g, h in zip(self.param_groups, groups):
+                mine, lr = g["lr"], float(h.get("lr", g["lr"]))
+                g.update({k: v for k, v in h.items() if k != "params"})
+                g["lr"] = mine.fill_(lr) if torch.is_tensor(mine) else lr   # (a captured step reads a tensor lr where it is)
+            self.seed = int(sd.get("seed", self.seed))
+        return take

@@ -640,14 +640,66 @@ class Trainer:
         m = dict(iter=self.iter, epoch=0)
         m.update(meta or {})
         sd = {k: v.detach().cpu() for k, v in self.model.state_dict().items()}
-        torch.save(dict(meta=m, state_dict=sd, optimizer=self.opt.state_dict()), path)
+        optimizer = self.opt.state_dict() if isinstance(self.opt, FlatAdamW) else self._in_model_order(self.opt.state_dict())
+        torch.save(dict(meta=m, state_dict=sd, optimizer=optimizer), path)
+
+    def _model_index(self):
+        """For each parameter of a MultiTensorAdamW in its own order: its place among the model's parameters."""
+        at = {id(p): i for i, p in enumerate(self.flat.all_params)}
+        return [at[id(p)] for g in self.opt.param_groups for p in g["params"]]
+
+    def _in_model_order(self, sd):
+        """A MultiTensorAdamW's state_dict as FlatAdamW writes its own: one group for each of the model's parameters, frozen ones
+        included, in named_parameters() order.  (8 bits: the entries are codes and their exponents.)"""
+        index, count = self._model_index(), len(self.flat.all_params)
+        group_of = {n: g for g in sd["param_groups"] for n in g["params"]}
+        hyper = lambda g: dict({k: g[k] for k in ("betas", "eps", "weight_decay")}, lr=float(g["lr"]), amsgrad=False,
+                               initial_lr=float(g.get("initial_lr", g["lr"])))
+        groups = [dict(hyper(sd["param_groups"][0]), params=[i]) for i in range(count)]
+        steps = self.opt.steps().tolist()
+        state = {}
+        for n, i in enumerate(index):
+            groups[i] = dict(hyper(group_of[n]), params=[i])
+            state[i] = {**{k: v.clone() for k, v in sd["state"][n].items()}, "step": torch.tensor(float(steps[n]))}
+        out = dict(state=state, param_groups=groups, parameter_order="model", **{k: sd[k] for k in ("state_bits", "master_weights", "seed")})
+        if "memory_orders" in sd:
+            out["memory_orders"] = [None] * count
+            for n, i in enumerate(index):
+                out["memory_orders"][i] = sd["memory_orders"][n]
+        return out
+
+    def _from_model_order(self, sd):
+        """... and back, from any state in that order (FlatAdamW's, mmcv's, torch.optim.AdamW's of model.parameters()).  As in FlatAdamW,
+        the learning rates are the state's, the other hyper-parameters this trainer's."""
+        if "state_bits" in sd and sd.get("parameter_order") != "model":
+            return sd                                                      # (the optimizer's own order)
+        index, count = self._model_index(), len(self.flat.all_params)
+        extra = [k for k in sd["state"] if not (isinstance(k, int) and 0 <= k < count)]
+        if extra:
+            raise ValueError(f"optimizer state has entries for parameters this model does not have: {extra[:4]}")
+        group_of = {i: g for g in sd["param_groups"] for i in g["params"]}
+        mine = self.opt.state_dict()["param_groups"]
+        groups = []
+        for g in mine:
+            theirs = group_of.get(index[g["params"][0]], {})
+            groups.append({**g, **{k: theirs[k] for k in ("lr", "initial_lr") if k in theirs}})
+        if any(g.get("amsgrad") or g.get("maximize") for g in sd["param_groups"]):
+            raise ValueError("amsgrad and maximize are not supported")
+        out = {**sd, "state": {n: sd["state"][i] for n, i in enumerate(index) if i in sd["state"]}, "param_groups": groups}
+        if "memory_orders" in sd:
+            out["memory_orders"] = [sd["memory_orders"][i] for i in index]
+        return out
 
     def load_checkpoint(self, path, strict=True):
         ck = torch.load(path, map_location="cpu", weights_only=False)
+        state = ck.get("optimizer")
+        if state:                                        # (a state that is refused is refused before the model is touched)
+            state = state if isinstance(self.opt, FlatAdamW) else self._from_model_order(state)
+            self.opt.check_state(state)
         self.model.load_state_dict(ck["state_dict"], strict=strict)        # parameters are views of the flat buffer
         self.flat.check_storage()
-        if ck.get("optimizer"):
-            self.opt.load_state_dict(ck["optimizer"])
+        if state:
+            self.opt.load_state_dict(state)
         if self.engine is not None:                      # the parameters and Adam's counter changed under the engine
             self.engine.invalidate_packed()
             self.engine.set_optimizer_steps(self.opt.step_count)

@@ -178,3 +178,79 @@ def test_pretraining_step_with_this_optimizer(dev):
     for tr in (a, b):
         losses, _ = tr.train_step(pts)
         assert all(np.isfinite(float(v)) for v in losses.values())
+
+
+class Small(torch.nn.Module):
+    """Decayed and undecayed parameters, one of them frozen, in an order that no optimizer's own is."""
+
+    def __init__(self):
+        super().__init__()
+        self.lin = torch.nn.Linear(6, 50)
+        self.norm = torch.nn.LayerNorm(50)
+        self.fixed = torch.nn.Parameter(torch.ones(3), requires_grad=False)
+        self.out = torch.nn.Linear(50, 50)
+        self.norm2 = torch.nn.LayerNorm(50)
+
+    def forward_train(self, points, img_metas=None, **kw):
+        return {"loss": (self.norm2(self.out(torch.relu(self.norm(self.lin(points))))) * torch.arange(50, device=points.device)).pow(2).mean()}
+
+
+def small_trainer(dev, typ, seed=0, **kw):
+    from geomae_amd.train import Trainer
+    torch.manual_seed(seed)
+    ocfg = dict(type=typ, lr=1e-2, weight_decay=0.05, paramwise_cfg=dict(custom_keys={"norm": dict(decay_mult=0.0)}), **kw)
+    return Trainer(Small().to(dev), ocfg, grad_clip=dict(max_norm=10.0, norm_type=2))
+
+
+def test_checkpoints_go_between_the_optimizers(dev, tmp_path):
+    """A trainer's checkpoint has the optimizer's state by the model's parameter order whatever the optimizer, so that a run with one
+    continues with the other; one that does not fit is refused before the model is touched."""
+    x = torch.randn(64, 6, device=dev, generator=torch.Generator(device=dev).manual_seed(0))
+    path = str(tmp_path / "c.pth")
+
+    def moments(tr, name):
+        if hasattr(tr.opt, "exp_avg"):
+            return [getattr(tr.opt, name)[o:o + p.numel()].view_as(p) for p, o in zip(tr.flat.params, tr.flat.offsets)]
+        return [tr.opt.state[p][name] for p in tr.flat.params]
+    for a, b in (("AdamW", "MultiTensorAdamW"), ("MultiTensorAdamW", "AdamW"), ("MultiTensorAdamW", "MultiTensorAdamW")):
+        one, two = small_trainer(dev, a), small_trainer(dev, b, seed=1)
+        for _ in range(3):
+            one.train_step(x)
+        one._set_lr(5e-3)
+        one.save_checkpoint(path)
+        ck = torch.load(path, weights_only=False)["optimizer"]
+        names = [n for n, _ in one.model.named_parameters()]
+        assert [g["params"] for g in ck["param_groups"]] == [[i] for i in range(len(names))] and set(ck["state"]) == set(range(len(names))) - {names.index("fixed")}
+        assert [g["weight_decay"] == 0.0 for g in ck["param_groups"]] == ["norm" in n for n in names]
+        two.load_checkpoint(path)
+        assert all(torch.equal(p, q) for p, q in zip(one.model.parameters(), two.model.parameters()))
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert all(torch.equal(p, q) for p, q in zip(moments(one, k), moments(two, k)))
+        one.train_step(x)
+        two.train_step(x)
+        # the same step in fp32 operations on both sides: 2^-24 of |p| and some of an update of at most lr / (1 - beta1) each
+        for p, q in zip(one.model.parameters(), two.model.parameters()):
+            assert float((p - q).abs().max()) <= 2 * 2.0 ** -24 * (4 * float(p.abs().max()) + 40 * 5e-2)
+    ref = torch.optim.AdamW([dict(params=[p]) for p in Small().to(dev).parameters()])     # torch's own takes it too
+    ref.load_state_dict(dict(ck, param_groups=[dict(g, maximize=False, foreach=None, capturable=False, differentiable=False, fused=None,
+                                                    decoupled_weight_decay=True) for g in ck["param_groups"]]))
+    for a, ka, b, kb in (("MultiTensorAdamW", dict(state_bits=8), "AdamW", {}), ("AdamW", {}, "MultiTensorAdamW", dict(state_bits=8))):
+        one, two = small_trainer(dev, a, **ka), small_trainer(dev, b, seed=1, **kb)
+        one.train_step(x)
+        one.save_checkpoint(path)
+        before = [p.detach().clone() for p in two.model.parameters()]
+        with pytest.raises(ValueError, match="bits"):
+            two.load_checkpoint(path)
+        assert all(torch.equal(p, q) for p, q in zip(two.model.parameters(), before)) and two.iter == 0
+    # 8 bits to 8 bits, and a state in the optimizer's own order, as it was written before
+    one, two, three = (small_trainer(dev, "MultiTensorAdamW", seed=s, state_bits=8) for s in (0, 1, 2))
+    for _ in range(2):
+        one.train_step(x)
+    one.save_checkpoint(path)
+    two.load_checkpoint(path)
+    ck = torch.load(path, weights_only=False)
+    torch.save(dict(ck, optimizer=one.opt.state_dict()), path)
+    three.load_checkpoint(path)
+    for tr in (one, two, three):
+        tr.train_step(x)
+    assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(one.flat.params, two.flat.params, three.flat.params))
