@@ -7,8 +7,8 @@
 // The sums of the statistics are in fp64, and mean and rstd are kept as fp64: their rounding moves every element of a group
 // together, an fp32 sum of squares loses a small variance under a large mean, and ReLU's border in the backward pass (is z
 // over zero?) is decided by a threshold on x that is worked out in fp64 and rounded so that no fp32 x lies between it and the
-// true one.  The rest is fp32; the gradient sums are fp32 within a workgroup's rows and fp64 across workgroups, always in the
-// same order.
+// true one.  The rest is fp32; the gradient sums are fp32 within a workgroup's rows, 256 of them one after the other at most, and fp64
+// across workgroups, always in the same order.
 //
 // A thread keeps to one vector of V neighbouring channels of one group (V = 4, 2 or 1, whichever divides cg first), so that its
 // statistics, gamma and beta stay in registers.  (8 channels of a 16-bit type, one access of 16 bytes, set up twice as much per
@@ -33,6 +33,7 @@ namespace geomae {
 constexpr int kGnThreads = 256;                    // of a streamed workgroup
 constexpr int kGnMaxGroups = 1024, kGnMaxChannels = 1 << 22;
 constexpr int kGnBlocks = 1024;                    // workgroups of a streamed pass: four per CU
+constexpr int kGnSumRows = 256;                    // rows that a thread adds up in fp32 (a multiple of the rows in flight)
 constexpr int kGnFold = 64;                        // samples whose sums one thread adds up for the parameters' gradients
 constexpr int kGnResidentThreads = 1024;
 
@@ -863,6 +864,8 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
     const int64_t least = (int64_t)ty * unroll, wanted = kGnBlocks / n > 1 ? kGnBlocks / n : 1;
     s.chunk_rows = (rows + wanted - 1) / wanted;
     s.chunk_rows = s.chunk_rows < least ? least : (s.chunk_rows + least - 1) / least * least;
+    // the gradient sums: a thread adds up at most kGnSumRows rows in fp32, whatever the batch leaves to a workgroup
+    if (backward && s.chunk_rows > (int64_t)kGnSumRows * ty) s.chunk_rows = (int64_t)kGnSumRows * ty;
     s.chunks = s.cs ? 0 : (int32_t)((rows + s.chunk_rows - 1) / s.chunk_rows);
     return s;
 }

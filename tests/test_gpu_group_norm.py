@@ -408,3 +408,16 @@ def test_columns_and_rows_of_a_workgroup(dev, shape, groups, dtype):
         got = run_both(x, groups, w, b, act, dy)
         for k in want:
             check(got[k], want[k], (act, k))
+
+
+def test_gradient_sums_do_not_lose_what_is_small(dev):
+    """Many samples, so that a workgroup has all rows of one: 1 and then 999 times half a unit of its last place.  Added one after the other
+    in fp32 they vanish (3e-5 of the sum); at most 300 additions in a row lose 300 h."""
+    n, rows, c = 1024, 1000, 131
+    x = torch.randn(n, rows, c, device=dev).movedim(-1, 1)
+    dy = torch.full((n, rows, c), 2.0 ** -25, device=dev)
+    dy[:, 0] = 1.0
+    w, b = torch.ones(c, device=dev), torch.zeros(c, device=dev)
+    got = run_both(x, 1, w, b, None, dy.movedim(-1, 1))
+    want = n * (1 + 999 * 2.0 ** -25)
+    assert float((got["dbias"].double() / want - 1).abs().max()) <= 300 * H
