@@ -4,8 +4,10 @@
 //   dz = dy act'(z);  dbeta = sum dz, dgamma = sum dz xhat over samples and rows
 //   dx = rstd (gamma dz - s1 - xhat s2),   s1, s2 = means over the group of gamma dz and of gamma dz xhat
 //
-// The sums of the statistics are in fp64, and mean and rstd are kept as fp64: their rounding moves every element of a group
-// together, an fp32 sum of squares loses a small variance under a large mean, and ReLU's border in the backward pass (is z
+// The sums of the statistics are in fp64, of the elements less the group's first one: sums of the squares themselves lose a small
+// variance under a large mean, in 64 bits too (a mean of 2^20 spreads leaves 2^-13 of it).  The first element is within sqrt(m var) of the
+// mean, m elements, so that the difference of the two sums is good to m 2^-53 of the variance at worst, and to some 2^-53 as a rule.
+// Mean and rstd are kept as fp64: their rounding moves every element of a group together, and ReLU's border in the backward pass (is z
 // over zero?) is decided by a threshold on x that is worked out in fp64 and rounded so that no fp32 x lies between it and the
 // true one.  The rest is fp32; the gradient sums are fp32 within a workgroup's rows, 256 of them one after the other at most, and fp64
 // across workgroups, always in the same order.
@@ -314,11 +316,12 @@ template <typename F> __device__ __forceinline__ void gn_each_group(int groups, 
 }
 __device__ __forceinline__ double gn_lanes_sum(double v, int lanes) { return lanes == 1 ? v : wave_sum(v); }
 
-__device__ __forceinline__ double2 gn_statistics(double sum, double sq, double inv_m, double eps) {
+// first: the group's first element, which was taken off the summed ones
+__device__ __forceinline__ double2 gn_statistics(double first, double sum, double sq, double inv_m, double eps) {
     const double mean = sum * inv_m;
     double var = sq * inv_m - mean * mean;
     var = var < 0.0 ? 0.0 : var;                                       // (NaN stays)
-    return make_double2(mean, 1.0 / sqrt(var + eps));
+    return make_double2(first + mean, 1.0 / sqrt(var + eps));
 }
 
 // ------------------------------------------------------------------------------------------------ resident
@@ -363,6 +366,9 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_forward_kernel
         const int r = l.row + u * l.ty;
         if (l.live && r < rows) v[u] = gn_read<T, V>(x + base + (int64_t)r * s.c);
     }
+    const int mine = (l.live ? l.col : 0) / s.cg;                      // this thread's group of the workgroup's
+    const T* const row0 = x + (int64_t)l.n * s.rows * s.c + l.c0;      // the sample's first row
+    const double first = (double)gn_float(row0[mine * s.cg]);
     GnScale<V> ch;
     ch.weights(w, l.c0 + (l.live ? l.col : 0));
     double a[2] = {0.0, 0.0};
@@ -371,7 +377,7 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_forward_kernel
         if (l.live && l.row + u * l.ty < rows) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const double d = (double)gn_float(v[u].v[i]);
+                const double d = (double)gn_float(v[u].v[i]) - first;
                 a[0] += d;
                 a[1] = fma(d, d, a[1]);
             }
@@ -387,13 +393,13 @@ __global__ __launch_bounds__(kGnResidentThreads) void gn_resident_forward_kernel
         sum = gn_lanes_sum(sum, lanes);
         sq = gn_lanes_sum(sq, lanes);
         if (lane == 0) {
-            group[g] = gn_statistics(sum, sq, s.inv_m, eps);
+            group[g] = gn_statistics((double)gn_float(row0[g * s.cg]), sum, sq, s.inv_m, eps);
             stats[(int64_t)l.n * s.groups + l.c0 / s.cg + g] = group[g];
         }
     });
     __syncthreads();
     if (!l.live) return;
-    ch.statistics(group[l.col / s.cg]);
+    ch.statistics(group[mine]);
     gn_by_act(act, [&](auto A) {
 #pragma unroll
         for (int u = 0; u < R; ++u) {
@@ -545,7 +551,7 @@ template <typename T, int V, int U, bool LAST = false, typename F> __device__ __
         if (l.row + u * l.ty < left) f(w[u], r * c + u * step);
 }
 
-// partial [n][groups][chunks]: (sum, sum of squares)
+// partial [n][groups][chunks]: (sum, sum of squares) of the elements less their group's first one
 template <typename T, int V>
 __global__ __launch_bounds__(kGnThreads) void gn_sums_kernel(const T* __restrict__ x, GnShape s, double2* __restrict__ partial) {
     __shared__ double lds[2 * kGnThreads], res[2 * kGnThreads];
@@ -558,15 +564,17 @@ __global__ __launch_bounds__(kGnThreads) void gn_sums_kernel(const T* __restrict
     for (int tile = 0; tile < tiles; ++tile) {
         const GnLanes l = gn_lanes<V>(s.c, tile);
         double a[2] = {0.0, 0.0};
-        if (l.live)
+        if (l.live) {
+            const double first = (double)gn_float(x[l.col / s.cg * s.cg]);
             gn_rows<T, V, gn_rows_in_flight(V)>(x, s.c, l, r0, r1, [&](const GnPack<T, V>& w, int64_t) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const double d = (double)gn_float(w.v[i]);
+                    const double d = (double)gn_float(w.v[i]) - first;
                     a[0] += d;
                     a[1] = fma(d, d, a[1]);
                 }
             });
+        }
         gn_sum_rows<double, 2>(a, l.tx, l.ty, res, lds);
         // columns -> the groups that begin in or reach into this tile
         const int per = s.cg / V, k0 = tile * kGnThreads, k1 = k0 + l.tx, g0 = k0 / per;
@@ -587,7 +595,9 @@ __global__ __launch_bounds__(kGnThreads) void gn_sums_kernel(const T* __restrict
 }
 
 // a wave per (sample, group): mean and 1 / sqrt(var + eps)
-__global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const double2* __restrict__ partial, GnShape s, double eps, double2* __restrict__ stats) {
+template <typename T>
+__global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restrict__ x, const double2* __restrict__ partial, GnShape s, double eps,
+                                                             double2* __restrict__ stats) {
     const int64_t at = (int64_t)blockIdx.x * (kGnThreads / kWave) + (threadIdx.x >> 6);
     if (at >= (int64_t)s.n * s.groups) return;
     double sum = 0.0, sq = 0.0;
@@ -599,7 +609,11 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const double2* __r
     }
     sum = wave_sum(sum);
     sq = wave_sum(sq);
-    if (lane_id() == 0) stats[at] = gn_statistics(sum, sq, s.inv_m, eps);
+    if (lane_id() == 0) {
+        const int64_t n = at / s.groups;
+        const double first = (double)gn_float(x[n * s.rows * s.c + (at - n * s.groups) * s.cg]);
+        stats[at] = gn_statistics(first, sum, sq, s.inv_m, eps);
+    }
 }
 
 template <typename T, int V>
@@ -988,7 +1002,7 @@ extern "C" int geomae_group_norm_forward(const void* x, int32_t dtype, int32_t n
         constexpr int V = decltype(vec)::value;
         const T* in = static_cast<const T*>(x);
         hipLaunchKernelGGL((gn_sums_kernel<T, V>), dim3(s.chunks * n), dim3(kGnThreads), groups * sizeof(double2), stream, in, s, ws.partial);
-        hipLaunchKernelGGL(gn_stats_kernel, dim3(cdiv((int64_t)n * groups, kGnThreads / kWave)), dim3(kGnThreads), 0, stream, ws.partial, s, eps, st);
+        hipLaunchKernelGGL(gn_stats_kernel<T>, dim3(cdiv((int64_t)n * groups, kGnThreads / kWave)), dim3(kGnThreads), 0, stream, in, ws.partial, s, eps, st);
         hipLaunchKernelGGL((gn_forward_kernel<T, V>), dim3(s.chunks * n), dim3(kGnThreads), 0, stream, in, s, st, w, activation, static_cast<T*>(y));
     });
     return check_launch("gn_forward_kernel");

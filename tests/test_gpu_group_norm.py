@@ -421,3 +421,20 @@ def test_gradient_sums_do_not_lose_what_is_small(dev):
     got = run_both(x, 1, w, b, None, dy.movedim(-1, 1))
     want = n * (1 + 999 * 2.0 ** -25)
     assert float((got["dbias"].double() / want - 1).abs().max()) <= 300 * H
+
+
+@pytest.mark.parametrize("shape", [(2, 16, 20, 20), (1, 16, 120, 120)], ids=["one launch", "three launches"])
+@pytest.mark.parametrize("mean", [2.0 ** 14, 2.0 ** 17, 2.0 ** 20])
+def test_a_mean_far_from_the_spread(dev, shape, mean):
+    """fp32 holds a spread of 1 beside 2^20 to four bits behind the point; the variance is that of what it holds, to the bounds of any other
+    input.  Also with the far element in the first place, which the sums are taken against, and in the last."""
+    x, dy, w, b = make(dev, shape, torch.float32)
+    far = channels_last(x + mean)
+    first, last = x.clone(memory_format=torch.preserve_format), x.clone(memory_format=torch.preserve_format)
+    first[:, ::4, 0, 0] = mean
+    last[:, 3::4, -1, -1] = -mean
+    for t in (far, first, last):
+        for act in (None, "relu"):
+            want, got = reference(t, 4, w, b, 1e-5, act, dy), run_both(t, 4, w, b, act, dy)
+            for k in want:
+                check(got[k], want[k], (act, k))
