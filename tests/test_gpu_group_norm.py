@@ -438,3 +438,41 @@ def test_a_mean_far_from_the_spread(dev, shape, mean):
             want, got = reference(t, 4, w, b, 1e-5, act, dy), run_both(t, 4, w, b, act, dy)
             for k in want:
                 check(got[k], want[k], (act, k))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_activations_keep_fp32s_digits(dev, act):
+    """fp32 over |z| up to 11, at the rounding of each operation and not of the activation's largest value.  The bound is the slope's share of
+    z's own 7 h |z| and the activation's operations (ulp = 2 h):
+      silu: z log2(e) rounds twice, of which the power makes 2 |z| h; exponential 2 h, sum h, reciprocal 2 h, product h: (6 + 2 |z|) h |y|
+      gelu: |z| density R: the exponent z^2 / 2 rounds three times: 1.5 z^2 h; exponential 2 h, two products 2 h; R = 1/2 - u Q, fit 1.1 h,
+            u and Q 6 h of up to 1/2, h / 2 of its own, and R (1 + |z|) is never below 0.4: 9 (1 + |z|) h; the last sum h |y|
+    In the 2-norm over z < -1, where the slope is small: no worse than the same in elementary fp32 operations and 2 h of z."""
+    rows, c = 64, 1024
+    gen = torch.Generator(device=dev).manual_seed(4)
+    x = torch.randn(rows, c, generator=gen, device=dev)
+    for scale in (1.0, 3.0):
+        w, b = torch.full((c,), scale, device=dev), torch.zeros(c, device=dev)
+        z = reference(x, 1, w, b, 1e-5, None)["y"][0].reshape(rows, c)
+        dy = torch.zeros(rows, c, device=dev)
+        dy[:, ::37] = 1.0                                                   # (dx of these is their slope's, less two small means)
+        got = run_both(x, 1, w, b, act, dy)
+        y, slope = act64(z, act)
+        err_z = H * (6 * z.abs() + z.abs())
+        a = z.abs()
+        if act == "gelu":
+            tail = 0.5 * torch.erfc(a / math.sqrt(2))
+            own = H * (y.abs() + a * tail * (6 + 1.5 * z * z + 9 * (1 + a)))
+        else:
+            own = H * y.abs() * (6 + 2 * a)
+        err = (got["y"].double() - y).abs()
+        assert float((err / (slope.abs() * err_z + err_z ** 2 + own)).max()) <= 1.0, (scale, act)
+        zf = z.float()
+        if act == "gelu":
+            plain = zf * (0.5 * (1 + torch.erf(zf * math.sqrt(0.5))))
+        else:
+            plain = zf / (1 + torch.exp(-zf))
+        low = z < -1
+        own_norm, plain_norm = (float((e[low] ** 2).sum().sqrt()) for e in (got["y"].double() - y, plain.double() - act64(zf.double(), act)[0]))
+        assert own_norm <= plain_norm + 2 * H * float((z * slope)[low].norm()), (scale, act, own_norm, plain_norm)
+        check(got["dx"], reference(x, 1, w, b, 1e-5, act, dy)["dx"])
