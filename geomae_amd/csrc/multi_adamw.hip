@@ -119,7 +119,7 @@ __device__ __forceinline__ uint32_t ma_code_root(const float (&x)[kMaVec], float
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < kMaVec; ++i) {
-        const uint32_t z = __float_as_uint(x[i] * scale * 0x1p-120f);
+        const uint32_t z = __float_as_uint(fabsf(x[i]) * scale * 0x1p-120f);               // (a NaN may have a sign)
         const uint32_t c = min(max((z + ((draw[i] >> 13 & ~7u) | 4u)) >> 19, min(__float_as_uint(x[i]), 1u)), 255u);
         w |= c << (8 * i);
     }

@@ -646,3 +646,23 @@ def test_the_first_step_is_the_same_in_8_bits(dev, eps):
         differ = (a != b) & ~a.isnan()
         assert int(differ.sum()) <= 1e-5 * n
         assert not differ.any() or float(((a - b).abs() / a.abs())[differ].max()) <= 4 * H
+
+
+def test_every_nan_is_held_as_one(dev):
+    """A NaN of any sign and payload in a gradient makes both moments NaN, whatever the draw, and nothing else of its block."""
+    for dtype, nans in ((torch.bfloat16, (0xffff, 0x7fff, 0xff81, 0x7f81)), (torch.float16, (0xffff, 0x7fff, 0xfc01, 0x7c01)),
+                        (torch.float32, (0xffffffff, 0x7fffffff, 0xff800001, 0x7f800001))):
+        n = 32 * 64 * len(nans)
+        p = torch.nn.Parameter(torch.zeros(n, device=dev, dtype=dtype))
+        grad = torch.ones(n, dtype=dtype)
+        raw = grad.numpy().view("uint16" if grad.element_size() == 2 else "uint32") if dtype != torch.bfloat16 else grad.view(torch.int16).numpy().view("uint16")
+        for k, bits in enumerate(nans):
+            raw[32 * k::32 * len(nans)] = bits
+        p.grad = grad.to(dev)
+        assert int(p.grad.isnan().sum()) == n // 32
+        opt = new([p], state_bits=8)
+        for _ in range(3):
+            opt.step()
+            m, r = opt.moments()
+            hit = p.grad.isnan()
+            assert m[hit].isnan().all() and r[hit].isnan().all() and m[~hit].isfinite().all() and r[~hit].isfinite().all()
