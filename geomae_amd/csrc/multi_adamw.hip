@@ -542,7 +542,9 @@ extern "C" int geomae_multi_adamw_step(const GeomaeAdamwTensor* table, const int
     const int64_t chunks_all = first_chunk[num_tensors];
     const bool norm = (max_norm > 0.0 || skip_nonfinite || grad_norm_out) && chunks_all > 0;
     pa.rows = table; pa.chunks = chunks; pa.scalars = w.scalars; pa.seed = seed;
-    pa.factor = {w.partial, 0, skip_nonfinite, grad_scale, grad_scale_ptr, (float)max_norm, nullptr};
+    // (a norm below fp32's numbers is not "no clipping")
+    const float limit = max_norm > 0.0 && (float)max_norm == 0.f ? 0x1p-149f : (float)max_norm;
+    pa.factor = {w.partial, 0, skip_nonfinite, grad_scale, grad_scale_ptr, limit, nullptr};
     pa.grad_norm = chunks_all == 0 ? grad_norm_out : nullptr;
     int32_t num_partial = 0;
     // skip_nonfinite: the scalars wait for the whole norm, a launch of their own

@@ -666,3 +666,12 @@ def test_every_nan_is_held_as_one(dev):
             m, r = opt.moments()
             hit = p.grad.isnan()
             assert m[hit].isnan().all() and r[hit].isnan().all() and m[~hit].isfinite().all() and r[~hit].isfinite().all()
+
+
+@pytest.mark.parametrize("max_norm", [1e-30, 1e-44, 1e-50])
+def test_the_smallest_norms_clip(dev, max_norm):
+    p = torch.nn.Parameter(torch.zeros(64, device=dev))
+    p.grad = torch.ones(64, device=dev)
+    opt = new([p])
+    opt.step(max_norm=max_norm)
+    assert float(opt.grad_norm) == 8.0 and float(opt.moments()[0].abs().max()) <= max_norm / 8 * 0.1 * 1.01 + 2.0 ** -149
