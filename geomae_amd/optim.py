@@ -315,7 +315,13 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         """A state_dict of this class with the same state_bits and masters, or (32 bits) one of torch.optim.AdamW.  Parameters
         that it has no state of begin anew; masters that it does not hold are taken from the parameters.  An 8-bit state of a parameter
         in another memory order (contiguous, now channels_last) is refused: its blocks are other elements here."""
+        sd = dict(sd)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            new = hook(self, sd)
+            sd = sd if new is None else new
         self.check_state(sd)()
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     def check_state(self, sd):
         """ValueError if load_state_dict() would refuse this state; else the function that takes it."""

@@ -675,3 +675,23 @@ def test_the_smallest_norms_clip(dev, max_norm):
     opt = new([p])
     opt.step(max_norm=max_norm)
     assert float(opt.grad_norm) == 8.0 and float(opt.moments()[0].abs().max()) <= max_norm / 8 * 0.1 * 1.01 + 2.0 ** -149
+
+
+def test_load_hooks_run(dev):
+    """As torch's optimizers: pre-hooks get a shallow copy and may change or replace it, post-hooks come after the load."""
+    params, _ = make(dev, torch.float32, [40])
+    opt = new(params)
+    opt.step()
+    sd, seen = opt.state_dict(), []
+
+    def replace(o, state):
+        seen.append(("pre", int(opt.state[params[0]]["step"])))
+        return {**state, "state": {0: {**state["state"][0], "step": torch.tensor(7)}}}
+    handles = [opt.register_load_state_dict_pre_hook(lambda o, state: state.__setitem__("seed", 5)), opt.register_load_state_dict_pre_hook(replace),
+               opt.register_load_state_dict_post_hook(lambda o: seen.append(("post", int(o.state[params[0]]["step"]))))]
+    opt.load_state_dict(sd)
+    assert seen == [("pre", 1), ("post", 7)] and opt.seed == 5 and sd["seed"] == 0
+    for h in handles:
+        h.remove()
+    opt.load_state_dict(sd)
+    assert len(seen) == 2 and int(opt.state[params[0]]["step"]) == 7 and opt.seed == 0
