@@ -7,6 +7,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <algorithm>
 #include "../../include/geomae_hip.h"
 
 namespace {
@@ -53,6 +54,8 @@ struct AdamwPlan {
     int state_bits;
     uint32_t seed;
     bool captured;                                                     // a captured step has these addresses
+    c10::SmallVector<geomaeStream_t, 2> streams;                       // that steps were enqueued on ...
+    bool new_stream;                                                   // ... the last one for the first time
     std::vector<const void*> grads;
     std::vector<int32_t> hyper_of;
     std::vector<c10::TensorImpl*> changed;
@@ -112,6 +115,7 @@ bool adamw_step(AdamwPlan& plan, py::list groups, double max_norm, double grad_s
     const at::NoGradGuard no_grad;
     const size_t n = plan.params.size();
     plan.changed.clear();
+    plan.new_stream = false;
     std::vector<GeomaeAdamwHyper> hypers;
     std::vector<at::Tensor> copies;
     c10::optional<c10::Device> device;
@@ -161,10 +165,13 @@ bool adamw_step(AdamwPlan& plan, py::list groups, double max_norm, double grad_s
         scale_ptr = scale_tensor->const_data_ptr<float>();
     }
     const c10::OptionalDeviceGuard guard(device);
+    const geomaeStream_t stream = stream_of(*device);
     check(lib.multi_adamw_step(plan.table, plan.chunks, plan.first_chunk.data(), (int32_t)n, plan.grads.data(), plan.hyper_of.data(), hypers.data(),
                                (int32_t)hypers.size(), plan.state_bits, max_norm, grad_scale, scale_ptr, skip_nonfinite, plan.seed,
-                               max_norm > 0.0 || skip_nonfinite ? plan.norm_word : nullptr, plan.workspace, plan.workspace_bytes, stream_of(*device)),
+                               max_norm > 0.0 || skip_nonfinite ? plan.norm_word : nullptr, plan.workspace, plan.workspace_bytes, stream),
           "geomae_multi_adamw_step");
+    plan.new_stream = std::find(plan.streams.begin(), plan.streams.end(), stream) == plan.streams.end();
+    if (plan.new_stream) plan.streams.push_back(stream);
     for (c10::TensorImpl* t : plan.changed) t->bump_version();         // the parameters changed, for autograd's saved tensors too
     plan.captured = plan.captured || c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
     return true;
@@ -364,13 +371,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             p.norm_word = reinterpret_cast<float*>(norm_word);
             p.state_bits = state_bits;
             p.seed = 0;
-            p.captured = false;
+            p.captured = p.new_stream = false;
             p.grads.resize(params.size());
             p.hyper_of.resize(params.size());
             return p;
         }))
         .def_readwrite("seed", &AdamwPlan::seed)
         .def_readonly("captured", &AdamwPlan::captured)
+        .def_readonly("new_stream", &AdamwPlan::new_stream)
         .def("step", &adamw_step);
     m.def("group_norm_act", &group_norm_act);
     m.def("accumulates_on_default_stream", &accumulates_on_default_stream);

@@ -122,6 +122,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise RuntimeError("MultiTensorAdamW: parameters cannot be added while a stream is captured")
         self._check_layout(params[:had])
         dev = params[0].device
+        torch.cuda.synchronize(dev)                 # (steps of any stream, whose state is copied below)
         offsets, total = [], 0
         for p in params:
             offsets.append(total)
@@ -152,6 +153,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         chunks = torch.stack([tensor, within.int()], 1).contiguous().to(dev)
         workspace = torch.empty(lib.geomae_multi_adamw_workspace_bytes(len(params)), dtype=torch.uint8, device=dev)
         norm_word = torch.zeros((), dtype=torch.float32, device=dev)
+        torch.cuda.synchronize(dev)                 # (the first step may be on any stream)
         self._set_table(params, arena, offsets, chunks, first, workspace, norm_word)
         self.state.update(zip(params, state))
 
@@ -239,6 +241,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             self._find_params()
             if not self._plan.step(self.param_groups, max_norm, scale, scale_tensor, skip_nonfinite):
                 raise RuntimeError("MultiTensorAdamW: the parameters moved during the step")
+        if self._plan.new_stream:                   # the caller knows nothing of these: their memory waits for this stream by itself
+            for t in (self._table, self._chunks, self._workspace, self._norm_word, *self._arena.values()):
+                t.record_stream(torch.cuda.current_stream(t.device))
         if max_norm > 0.0 or skip_nonfinite:
             self.grad_norm = self._norm_word
         return loss

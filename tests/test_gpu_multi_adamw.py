@@ -7,6 +7,8 @@ Bounds, with h = 2^-24 (half a step of fp32), counted operation by operation:
   p' = p (1 - lr wd) - u:                3 h |p| + h |p'| + err(u)        and half a step of the parameter's own type if that is 16 bits
 An 8-bit moment is the definition's code unless the position is nearer to the draw's border than the moment's own fp32 error
 (in steps); then its neighbour will do."""
+import gc
+
 import adamw_definition as D
 import numpy as np
 import pytest
@@ -695,3 +697,42 @@ def test_load_hooks_run(dev):
         h.remove()
     opt.load_state_dict(sd)
     assert len(seen) == 2 and int(opt.state[params[0]]["step"]) == 7 and opt.seed == 0
+
+
+def test_buffers_outlive_steps_on_other_streams(dev):
+    """The moments, the table and the workspace are the optimizer's own: made on one stream, stepped on a second at once, and dropped while
+    that step is still to run, they are neither read before they are there nor given to somebody else."""
+    side = torch.cuda.Stream()
+    for drop in ("optimizer", "table", "group"):
+        params, _ = make(dev, torch.float32, [40_000, 77])
+        twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+        for p, q in zip(params, twins):
+            q.grad = p.grad
+        want = new(twins)
+        want.step()
+        torch.cuda.synchronize()
+        torch.cuda._sleep(20_000_000)
+        opt = new(params)
+        sizes = [t.numel() for t in opt._arena.values()] + [opt._table.numel() // 4, opt._chunks.numel(), opt._workspace.numel() // 4]
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)
+            opt.step()
+        if drop == "optimizer":
+            del opt
+            gc.collect()
+        elif drop == "table":
+            kept = params[1].data                                          # (the parameter's memory is the caller's)
+            params[1].data = kept.clone()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                opt.step()
+            want.step()
+        else:
+            opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(9, device=dev))]})
+            with torch.cuda.stream(side):
+                opt.step()
+            want.step()
+        other = [torch.full((n,), float("nan"), device=dev) for n in sizes for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(params[0], twins[0]) and (drop == "table" or torch.equal(params[1], twins[1]))
+        assert all(t.isnan().all() for t in other)
