@@ -1024,7 +1024,11 @@ extern "C" int geomae_group_norm_backward(const void* x, const void* dy, int32_t
                                           const void* gamma, const void* beta, int32_t weight_dtype, int32_t activation, const double* stats,
                                           void* dx, void* dgamma, void* dbeta, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
     if (int rc = gn_check("group_norm_backward", n, rows, c, groups, dtype, weight_dtype, activation)) return rc;
-    if (n == 0 || rows == 0) return GEOMAE_OK;
+    if (n == 0 || rows == 0) {                                          // sums of nothing
+        if (!dgamma && !dbeta) return GEOMAE_OK;
+        hipLaunchKernelGGL(gn_weight_grad_kernel, dim3(cdiv(c, kGnThreads)), dim3(kGnThreads), 0, stream, nullptr, 0, c, weight_dtype, dgamma, dbeta);
+        return check_launch("gn_weight_grad_kernel");
+    }
     GEOMAE_REQUIRE(x && dy && stats && dx, "group_norm_backward: null argument");
     const GnShape s = gn_shape(n, rows, c, groups, dtype, activation, true);
     if (int rc = gn_check_launches("group_norm_backward", s)) return rc;

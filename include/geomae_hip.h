@@ -822,7 +822,7 @@ int geomae_adamw_moments8(const uint8_t* exp_avg, const uint8_t* exp_avg_exponen
  * x, y, dy, dx: [n][rows][c] of `dtype` (GEOMAE_DTYPE_*); a group is c / groups neighbouring channels of a sample (at most
  * 1024 groups and 2^22 channels).  y = act(gamma (x - mean) / sqrt(var + eps) + beta), var biased; gamma, beta [c] of weight_dtype, or NULL (1, 0).
  * stats [n][groups][2] fp64 (16-byte aligned) receives (mean, 1 / sqrt(var + eps)): the backward pass reads it.  dgamma, dbeta [c] of
- * weight_dtype, or NULL.  ReLU's derivative at 0 is 0; gelu is the erf form.  workspace: the forward and the backward pass need
+ * weight_dtype, or NULL (n or rows 0: zeros).  ReLU's derivative at 0 is 0; gelu is the erf form.  workspace: the forward and the backward pass need
  * geomae_group_norm_workspace_bytes(..., backward = 0 / 1) bytes each (-1: bad shape), 16-byte aligned. */
 enum { GEOMAE_ACT_NONE = 0, GEOMAE_ACT_RELU = 1, GEOMAE_ACT_SILU = 2, GEOMAE_ACT_GELU = 3 };
 int64_t geomae_group_norm_workspace_bytes(int32_t n, int64_t rows, int32_t c, int32_t groups, int32_t dtype, int32_t backward);

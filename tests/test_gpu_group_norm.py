@@ -476,3 +476,16 @@ def test_activations_keep_fp32s_digits(dev, act):
         own_norm, plain_norm = (float((e[low] ** 2).sum().sqrt()) for e in (got["y"].double() - y, plain.double() - act64(zf.double(), act)[0]))
         assert own_norm <= plain_norm + 2 * H * float((z * slope)[low].norm()), (scale, act, own_norm, plain_norm)
         check(got["dx"], reference(x, 1, w, b, 1e-5, act, dy)["dx"])
+
+
+def test_entry_point_without_rows_zeroes_the_weights_gradients(dev):
+    from geomae_amd import _lib
+    lib, stream = _lib.load(), torch.cuda.current_stream(dev).cuda_stream
+    for n, rows in ((0, 10), (3, 0)):
+        for k, dtype in enumerate((torch.float32, torch.bfloat16, torch.float16)):
+            for which in ((1, 1), (1, 0), (0, 1)):
+                grads = [torch.full((600,), 5.0, device=dev, dtype=dtype) for _ in range(2)]
+                ptrs = [t.data_ptr() if w else None for t, w in zip(grads, which)]
+                assert lib.geomae_group_norm_backward(None, None, 0, n, rows, 600, 2, None, None, k, 0, None, None, *ptrs, None, 0, stream) == 0
+                torch.cuda.synchronize()
+                assert all(not t.any() if w else (t == 5.0).all() for t, w in zip(grads, which))
