@@ -14,7 +14,7 @@
 //
 // A thread keeps to one vector of V neighbouring channels of one group (V = 4, 2 or 1, whichever divides cg first), so that its
 // statistics, gamma and beta stay in registers.  (8 channels of a 16-bit type, one access of 16 bytes, set up twice as much per
-// thread for half as many rows: 2 x 256 x 128 x 128 bf16 forward 22 us against 17.)  Two forms:
+// thread for half as many rows: a quarter longer at 2 x 256 x 128 x 128 bf16 forward, which takes 23 us.)  Two forms:
 //  resident  all rows of one or more groups fit a workgroup's registers (128 bytes a thread, 1024 threads: 4096 rows of 32
 //            bytes): x and dy are read once and one launch does a pass (the backward pass one more for the parameters'
 //            gradients if there is more than one sample).  Bound by launch, load latency and the workgroup's reductions (1 x 256 x
@@ -838,26 +838,48 @@ __global__ __launch_bounds__(kGnThreads) void gn_backward_kernel(const T* __rest
 }
 
 // ------------------------------------------------------------------------------------------------ host
+// Estimates of a pass in us for the choice of its form: linear in what each form does, fitted to 15000 random cases of 1 to 16384 samples,
+// 1 to 11600 rows, 16 to 512 channels, all types and activations, at which both forms were timed.  (256 CUs; a 1024-thread workgroup of
+// 128 registers fills one.)
+struct GnEstimate {
+    double one;                                    // a pass
+    // resident: a round of workgroups over the CUs, in it 1000 elements of a workgroup (silu, gelu: more), 1000 lines of 128 bytes that its
+    // rows touch, and columns that no wave holds whole; 10^6 lines, MB and 1000 waves of all
+    double round, elements, silu, gelu, lines, ragged, all_lines, mb, waves;
+    // streamed: MB, 10^6 elements (silu, gelu, one channel a thread: more), KB of a row, 1000 groups and 10^6 channels of all samples
+    double s_one, s_mb, s_elements, s_silu, s_gelu, s_single, s_row, s_groups, s_channels;
+};
+static const GnEstimate kGnEstimate[2] = {
+    {2.8, 1.7, 0.11, 0.029, 0.097, 0.71, 0.51, 3.2, 0.10, 0.35, 10.0, 0.28, 0.44, 0.09, 0.42, 0.90, 0.38, 0.3, 8.6},       // forward
+    {3.8, 3.3, 0.17, 0.075, 0.20, 0.80, 0.70, 3.3, 0.39, 0.64, 12.0, 0.38, 0.93, 0.24, 0.75, 0.03, 1.6, 4.0, 42.0}};       // backward
+static bool gn_streamed_fits(const GnShape& s) { return (int64_t)s.n * s.groups * kGnStatThreads <= UINT32_MAX; }
+static bool gn_streamed_is_faster(const GnShape& s, int item, int act, bool backward) {
+    const GnEstimate& e = kGnEstimate[backward];
+    const double workgroups = (double)s.n * s.slabs, waves = s.threads / kWave, at_once = 256.0 * (16 / (s.threads / kWave));
+    const double rounds = ceil(workgroups / at_once), own = 1e-3 * (double)s.rows * s.cs, lines = 1e-3 * (double)s.rows * ((s.cs * item + 127) / 128);
+    const double all = 1e-6 * (double)s.n * s.rows * s.c;
+    const double resident = e.one + rounds * (e.round + own * (e.elements + (act == kGnSilu ? e.silu : act == kGnGelu ? e.gelu : 0.0)) + lines * e.lines +
+                                              (gn_whole_rows(s.tx) ? 0.0 : e.ragged)) +
+                            1e-3 * workgroups * (lines * e.all_lines + waves * e.waves) + all * item * e.mb;
+    const double streamed = e.s_one + all * (item * e.s_mb + e.s_elements + (act == kGnSilu ? e.s_silu : act == kGnGelu ? e.s_gelu : 0.0) +
+                                             (s.v == 1 ? e.s_single : 0.0)) +
+                            1e-3 * s.c * item * e.s_row + 1e-3 * s.n * s.groups * e.s_groups + 1e-6 * (double)s.n * s.c * e.s_channels;
+    return streamed < resident;
+}
 static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int dtype, int act, bool backward) {
     GnShape s;
     s.n = n; s.rows = rows; s.c = c; s.groups = groups; s.cg = c / groups;
     s.inv_m = 1.0 / ((double)rows * s.cg);
     s.v = s.cg % 4 == 0 ? 4 : (s.cg % 2 == 0 ? 2 : 1);
-    s.past_cache = (double)n * rows * c * (dtype == GEOMAE_DTYPE_F32 ? 4 : 2) > 64e6;
     const int item = dtype == GEOMAE_DTYPE_F32 ? 4 : 2;
-    // Resident, if all rows of a group fit (fp32 forward: 8 x 512 x 20 x 20 6.5 us against 10.8 streamed, 4 x 256 x 50 x 50 11.0 against
-    // 13.8, 2 x 256 x 64 x 64 11.1 against 12.3); more groups to a workgroup while its piece of a row is short of a cache line and there
-    // are workgroups for every CU without.  Streamed for more than 4096 rows, whose pieces are a fraction of each line that is fetched
-    // (8 x 256 x 90 x 90 fp32 in groups of 4 channels: 42 us resident, 38 streamed; 4 x 128 x 100 x 100 bf16: 19 against 16), and where
-    // one workgroup a CU wastes what three launches cost:
-    //  many rows (a line each) of small pieces, or of tensors over 64 MB (backward: 8 x 64 x 64 x 64 bf16 in groups of 2 19.0 against
-    //  14.9; 16 x 256 x 64 x 64 fp32 73 against 62, forward 44 against 37);
-    //  many rows and CUs that have no workgroup, or none in the last round (backward: 2 x 256 x 64 x 64 fp32 25 against 19, 3 x 90 x 61 x 47
-    //  fp16 18 against 13, 24 x 256 x 64 x 64 bf16, 384 workgroups, 72 against 62, forward 40 against 33; 4 x 256 x 50 x 50 fp32 20 against 21);
-    //  silu and gelu, if the workgroups of a part of the CUs compute much (4 x 384 x 40 x 40 bf16 in groups of 24, gelu backward: 24.5
-    //  against 21.1, relu 17.2 against 21.0).
-    // Over 475 shapes of 1 to 16 samples, 400 to 4096 rows and 64 to 256 channels and three activations the form chosen takes 0.4 %
-    // (forward) and 0.7 % (backward) longer than the better one, always resident 1.4 and 6 %.
+    s.past_cache = (double)n * rows * c * item > 64e6;
+    // Resident, if all rows of a group fit and the estimates are for it; more groups to a workgroup while its piece of a row is short of a
+    // cache line and there are workgroups for every CU without.  Tensors over 64 MB of more than 1000 rows are streamed (46 cases forward and 46
+    // backward: resident 48 and 44 % longer than the better form, streamed 0.1).  Over 5000 random cases that the estimates were
+    // not fitted to (profiles/group_norm_forms.txt) the form chosen takes 0.9 % (forward) and 0.8 % (backward) longer than the better
+    // one, always resident where it fits 7.0 and 6.5, always streamed 64 and 57.  In us, resident against streamed, fp32 with ReLU: 8 x 512 x 20 x
+    // 20 forward 7.0 and 12.4, 4 x 256 x 50 x 50 backward 19.7 and 21.8; 2 x 256 x 64 x 64 backward (64 workgroups) 25.4 and 19.8, 8 x
+    // 256 x 90 x 90 in groups of 4 channels (an eighth of each line) forward 59 and 39.
     s.cs = s.threads = s.tx = s.ty = s.slabs = s.slab_groups = 0;
     s.tx_inverse = 0;
     const int held = gn_vectors_held(s.v, item);
@@ -865,18 +887,11 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
         const int64_t tx = cs / s.v;
         return tx <= kGnResidentThreads && rows <= kGnResidentThreads / tx * held;
     };
-    if (fits(s.cg) && rows <= 4096) {
+    if (fits(s.cg)) {
         int k = 1;
         for (int d = 2; d <= groups && (int64_t)k * s.cg * item < 128; ++d)
             if (groups % d == 0 && fits((int64_t)d * s.cg) && (int64_t)n * (groups / d) >= 256) k = d;
-        const int64_t workgroups = (int64_t)n * (groups / k), elements = rows * k * s.cg;
-        const bool idle = workgroups < (workgroups + 255) / 256 * 200;  // a fifth of the CUs and more, at least in the last round
-        const bool many_rows = rows > 2600 && (s.past_cache || (backward ? idle || k * s.cg * item < 16 : idle && workgroups > 256));
-        const bool much_work = (act == kGnGelu || act == kGnSilu) &&
-                               (backward ? idle && elements > 14000 : workgroups < 128 && elements > (act == kGnGelu ? 24000 : 48000));
-        s.cs = many_rows || much_work ? 0 : k * s.cg;
-    }
-    if (s.cs) {
+        s.cs = k * s.cg;
         const int64_t tx = s.cs / s.v;
         // (two vectors a thread: enough loads in flight, and half the threads to add up)
         int64_t threads = (tx * ((rows + 1) / 2) + kWave - 1) / kWave * kWave;
@@ -885,6 +900,7 @@ static GnShape gn_shape(int32_t n, int64_t rows, int32_t c, int32_t groups, int 
         s.threads = (int32_t)threads;
         s.tx = (int32_t)tx; s.ty = (int32_t)(threads / tx); s.slabs = c / s.cs; s.slab_groups = s.cs / s.cg;
         s.tx_inverse = (uint32_t)(((1 << 20) + tx - 1) / tx);
+        if (gn_streamed_fits(s) && ((s.past_cache && rows > 1000) || gn_streamed_is_faster(s, item, act, backward))) s.cs = 0;
     }
     const int cv = c / s.v, ty = cv < kGnThreads ? kGnThreads / cv : 1, unroll = gn_rows_in_flight(s.v);
     const int64_t least = (int64_t)ty * unroll, wanted = kGnBlocks / n > 1 ? kGnBlocks / n : 1;
@@ -975,7 +991,7 @@ extern "C" int64_t geomae_group_norm_workspace_bytes(int32_t n, int64_t rows, in
     if (gn_check("group_norm_workspace_bytes", n, rows, c, groups, dtype, 0, 0)) return -1;
     if (n == 0 || rows == 0) return 0;
     int64_t bytes = 0;
-    for (int act : {kGnNone, kGnGelu}) {                               // (the form may depend on the activation)
+    for (int act : {kGnNone, kGnSilu, kGnGelu}) {                      // (the form may depend on the activation)
         const GnShape s = gn_shape(n, rows, c, groups, dtype, act, backward != 0);
         if (gn_check_launches("group_norm_workspace_bytes", s)) return -1;
         const GnWorkspace w = gn_workspace(nullptr, s);
