@@ -489,3 +489,28 @@ def test_entry_point_without_rows_zeroes_the_weights_gradients(dev):
                 assert lib.geomae_group_norm_backward(None, None, 0, n, rows, 600, 2, None, None, k, 0, None, None, *ptrs, None, 0, stream) == 0
                 torch.cuda.synchronize()
                 assert all(not t.any() if w else (t == 5.0).all() for t, w in zip(grads, which))
+
+
+def test_one_and_two_channels_a_thread_past_the_caches(dev):
+    """Over 64 MB in groups whose channels divide by 2 or not at all: accesses of one and two elements that leave the caches."""
+    for dtype, c, groups in ((torch.float32, 33, 3), (torch.float32, 42, 7), (torch.bfloat16, 70, 7), (torch.float16, 66, 6)):
+        x, dy, w, b = make(dev, (1, c, 701, 701), dtype)
+        assert x.numel() * x.element_size() > 64e6 and (c // groups) % 4
+        want, got = reference(x, groups, w, b, 1e-5, "silu", dy), run_both(x, groups, w, b, "silu", dy)
+        for k in want:
+            check(got[k], want[k], (dtype, k))
+
+
+def test_definition_is_torchs():
+    """The 64-bit definition above against torch's group norm and activations, gradients included, on the CPU."""
+    import torch.nn.functional as F
+    gen = torch.Generator().manual_seed(0)
+    x, dy = (torch.randn(3, 24, 5, 7, generator=gen, dtype=torch.float64) for _ in range(2))
+    w, b = (torch.randn(24, generator=gen, dtype=torch.float64) for _ in range(2))
+    for act, f in ((None, lambda z: z), ("relu", F.relu), ("silu", F.silu), ("gelu", F.gelu)):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        y = f(F.group_norm(leaves[0], 6, leaves[1], leaves[2], 1e-3))
+        theirs = dict(zip(("y", "dx", "dweight", "dbias"), (y, *torch.autograd.grad(y, leaves, dy))))
+        mine = reference(x, 6, w, b, 1e-3, act, dy)
+        for k, t in theirs.items():
+            assert torch.allclose(mine[k][0].reshape(t.shape), t.detach(), rtol=1e-11, atol=1e-12), (act, k)
