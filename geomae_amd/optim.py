@@ -62,6 +62,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         self._arena, self._building, self._plan, self._layout, self._retired = None, True, None, [], []
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        if not self._params():
+            raise ValueError("MultiTensorAdamW: no parameter in any group")
         self._building = False
         self._build()
 
@@ -92,7 +94,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise
 
     def _check_params(self, params):
-        first = self.param_groups[0]["params"][0]
+        if not self._params():
+            return                                  # (a group without parameters, e.g. of a model without biases; the next ones have some)
+        first = self._params()[0]
         if len({id(p) for p in params}) != len(params):
             raise ValueError("MultiTensorAdamW: a parameter is listed twice")
         for p in params:

@@ -736,3 +736,20 @@ def test_buffers_outlive_steps_on_other_streams(dev):
         torch.cuda.synchronize()
         assert torch.equal(params[0], twins[0]) and (drop == "table" or torch.equal(params[1], twins[1]))
         assert all(t.isnan().all() for t in other)
+
+
+def test_groups_without_parameters(dev):
+    """A group may be empty, the first one too, as with torch's optimizers (a model without biases, everything frozen in one of them)."""
+    params, _ = make(dev, torch.float32, [40, 33])
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    for p, q in zip(params, twins):
+        q.grad = p.grad
+    a = new([{"params": [], "weight_decay": 0.0}, {"params": params[:1]}, {"params": []}, {"params": params[1:], "lr": 1e-2}])
+    b = new([{"params": twins[:1]}, {"params": twins[1:], "lr": 1e-2}])
+    for o in (a, b):
+        o.step(max_norm=0.1)
+    a.add_param_group({"params": []})
+    a.load_state_dict(a.state_dict())
+    for o in (a, b):
+        o.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, twins)) and len(a.param_groups) == 5

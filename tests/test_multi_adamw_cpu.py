@@ -136,3 +136,10 @@ def test_memory_orders():
     assert _memory_order(torch.empty(3, 4).t()) == [1, 0] and _memory_order(torch.empty(())) == [] == _memory_order(torch.empty(0, 4))
     one = torch.empty(6, 1, 5, 1)                                         # dimensions of one element do not count
     assert _memory_order(one) == [0, 2] == _memory_order(one.to(memory_format=torch.channels_last))
+
+
+def test_no_parameter_at_all_is_refused():
+    from geomae_amd.optim import MultiTensorAdamW
+    for none in ([{"params": []}], [{"params": []}, {"params": []}], []):
+        with pytest.raises(ValueError, match="no parameter|empty parameter list"):
+            MultiTensorAdamW(none)
