@@ -124,7 +124,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         params, had = self._params(), len(self._layout)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("MultiTensorAdamW: parameters cannot be added while a stream is captured")
-        self._check_layout(params[:had])
+        if had:
+            self._check_layout([p for g in self.param_groups[:-1] for p in g["params"]])
         dev = params[0].device
         torch.cuda.synchronize(dev)                 # (steps of any stream, whose state is copied below)
         offsets, total = [], 0
@@ -206,9 +207,12 @@ class MultiTensorAdamW(torch.optim.Optimizer):
 
     @staticmethod
     def _layouts(params):
-        return [(p.shape, p.stride(), p.dtype, p.device) for p in params]
+        return [(id(p), p.shape, p.stride(), p.dtype, p.device) for p in params]
 
     def _check_layout(self, params):
+        if [l[0] for l in self._layouts(params)] != [l[0] for l in self._layout]:
+            raise RuntimeError("MultiTensorAdamW: a parameter was replaced, removed or moved in its groups (the moments would be another's); "
+                               "make a new optimizer")
         if self._layouts(params) != self._layout:
             raise RuntimeError("MultiTensorAdamW: a parameter changed its shape, layout, dtype or device; make a new optimizer")
 
@@ -240,6 +244,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         max_norm = float(max_norm or 0.0)
         if not max_norm >= 0.0:
             raise ValueError(f"max_norm must not be negative, got {max_norm}")
+        if len(self.state) != len(self._layout):
+            raise RuntimeError("MultiTensorAdamW: the state was cleared or replaced, which does not reach the moments; load a state_dict (one with an "
+                               "empty state begins anew)")
         self._plan.seed = self.seed
         if not self._plan.step(self.param_groups, max_norm, scale, scale_tensor, skip_nonfinite):
             self._find_params()

@@ -753,3 +753,35 @@ def test_groups_without_parameters(dev):
     for o in (a, b):
         o.step()
     assert all(torch.equal(p, q) for p, q in zip(params, twins)) and len(a.param_groups) == 5
+
+
+def test_parameters_and_state_replaced_behind_the_optimizer(dev):
+    """A parameter object replaced by another of its shape, two swapped, one removed, the state cleared: a step would use another's moments, or
+    ones that the caller thinks are gone.  Each is refused and changes nothing; a state_dict with an empty state does begin anew."""
+    import collections
+    params = [torch.nn.Parameter(torch.randn(64, device=dev)) for _ in range(3)]
+    for p in params:
+        p.grad = torch.randn_like(p)
+    opt = new(params)
+    opt.step()
+    held, before = list(params), [p.detach().clone() for p in params]
+    other = torch.nn.Parameter(params[1].detach().clone())
+    other.grad = params[1].grad
+    group = opt.param_groups[0]
+    for wrong in ([held[0], other, held[2]], [held[1], held[0], held[2]], held[:2], held + [other]):
+        group["params"] = wrong
+        with pytest.raises(RuntimeError, match="make a new optimizer"):
+            opt.step()
+        with pytest.raises(RuntimeError, match="make a new optimizer"):
+            opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4, device=dev))]})
+    group["params"] = held
+    state = opt.state
+    opt.state = collections.defaultdict(dict)
+    with pytest.raises(RuntimeError, match="state was cleared"):
+        opt.step()
+    opt.state = state
+    assert all(torch.equal(p, q) for p, q in zip(held, before)) and (opt._arena["step"] == 1).all()
+    opt.load_state_dict({**opt.state_dict(), "state": {}})
+    assert not opt.moments()[0].any() and not opt._arena["step"].any()
+    opt.step()
+    assert (opt._arena["step"] == 1).all()
