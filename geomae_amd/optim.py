@@ -244,7 +244,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         max_norm = float(max_norm or 0.0)
         if not max_norm >= 0.0:
             raise ValueError(f"max_norm must not be negative, got {max_norm}")
-        if len(self.state) != len(self._layout):
+        if len(self.state) < len(self._layout):
             raise RuntimeError("MultiTensorAdamW: the state was cleared or replaced, which does not reach the moments; load a state_dict (one with an "
                                "empty state begins anew)")
         self._plan.seed = self.seed

@@ -345,6 +345,9 @@ class FlatAdamW:
         """ValueError if load_state_dict() would refuse this state."""
         if int(sd.get("state_bits", 32)) != 32:
             raise ValueError(f"the optimizer state holds moments in {sd['state_bits']} bits, this optimizer in 32")
+        if "state_bits" in sd and sd.get("parameter_order") != "model" and len(sd["param_groups"]) > 1:
+            raise ValueError("the state of a MultiTensorAdamW with several groups is in the order of its groups, not the model's: load it into one, "
+                             "whose trainer writes it in the model's order")
         order = self._checkpoint_order()
         extra = [k for k in sd["state"] if not (isinstance(k, int) and 0 <= k < len(order))]
         if extra:

@@ -785,3 +785,12 @@ def test_parameters_and_state_replaced_behind_the_optimizer(dev):
     assert not opt.moments()[0].any() and not opt._arena["step"].any()
     opt.step()
     assert (opt._arena["step"] == 1).all()
+
+
+def test_state_may_hold_other_entries(dev):
+    p = torch.nn.Parameter(torch.ones(8, device=dev))
+    p.grad = torch.ones(8, device=dev)
+    opt = new([p])
+    opt.state["count"] = 3                                                 # (torch's optimizers take it too)
+    opt.step()
+    assert int(opt.state[p]["step"]) == 1

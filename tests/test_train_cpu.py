@@ -334,3 +334,21 @@ def test_flat_adamw_refuses_codes_and_a_refused_state_changes_nothing():
         assert torch.equal(opt.exp_avg, kept[0]) and torch.equal(opt.exp_avg_sq, kept[1]) and opt.step_count == 0
     opt.load_state_dict(dict(good, state=other))
     assert opt.step_count == 3 and all((opt.exp_avg[o:o + p.numel()] == 1).all() for p, o in zip(flat.params, flat.offsets))
+
+
+def test_flat_adamw_refuses_a_state_in_the_order_of_groups():
+    """Same shapes at other places: a state in the order [decayed | undecayed] would go to other parameters without an error."""
+    class Square(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.norm, self.a = nn.Parameter(torch.ones(4)), nn.Parameter(torch.ones(4))
+    opt = FlatAdamW(FlatParams(Square(), no_decay_keys=("norm",)))
+    entry = lambda v: dict(step=torch.tensor(1), exp_avg=torch.full((4,), v), exp_avg_sq=torch.full((4,), v))
+    groups = [dict(params=[0], lr=1e-3), dict(params=[1], lr=1e-3)]
+    state = dict(state={0: entry(1.0), 1: entry(2.0)}, param_groups=groups, state_bits=32, master_weights=False, seed=0)
+    with pytest.raises(ValueError, match="order of its groups"):
+        opt.load_state_dict(state)
+    assert not opt.exp_avg.any() and opt.step_count == 0
+    opt.load_state_dict(dict(state, parameter_order="model"))
+    assert (opt.exp_avg[opt.flat.offsets[opt.flat.names.index("a")]:][:4] == 2.0).all()
+    opt.load_state_dict(dict(state, param_groups=[dict(params=[0, 1], lr=1e-3)]))
