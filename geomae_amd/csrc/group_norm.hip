@@ -23,7 +23,7 @@
 //            that writes.  Bound by HBM, or the 256 MB cache that the second read of x and dy comes from where they fit in it.
 //            Tensors over 64 MB: the writing pass loads and stores past the caches (4 x 128 x 200 x 200 fp32, both passes 132 ->
 //            117 us; 61 M bf16 elements forward 84 -> 67 us); smaller ones stay there for whoever comes next.  The launches of 4 x 128 x
-//            200 x 200 fp32 (82 MB a tensor): sums 17 us (4.9 TB/s), writing 25 (6.6), gradient sums 31 (5.3), gradients 37 (6.7), the two
+//            200 x 200 fp32 (82 MB a tensor): sums 17 us (4.7 TB/s), writing 24 (6.8), gradient sums 31 (5.3), gradients 36 (6.8), the two
 //            launches between them 4.6 each.
 #include "common.h"
 #include "../../include/geomae_hip.h"

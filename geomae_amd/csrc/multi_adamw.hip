@@ -20,8 +20,9 @@
 // What bounds it: HBM.  Bytes per element: fp32 parameters 28 with 32-bit moments (p, m, v in and out, g in) and 16 1/8 with
 // 8-bit ones.  A workgroup takes a chunk of 4096 elements of one tensor, found through a table built once; the gradients'
 // addresses, which change from step to step, ride in the launch's arguments, so that no copy to the device and no state of the
-// call's own stands between two steps or inside a captured graph.  Measured: 40 M fp32 elements, 32-bit moments 214 us (1.12 GB, 5.2
-// TB/s); 48 M bf16 elements with masters, 8-bit moments 140 us (0.77 GB, 5.5 TB/s) and 33 us for the norm before it (96 MB, 2.9 TB/s).
+// call's own stands between two steps or inside a captured graph.  Measured on two cards: 40 M fp32 elements, 32-bit moments 200 and 215 us
+// (1.12 GB, 5.6 and 5.2 TB/s, as a copy of as many bytes); 48 M bf16 elements with masters, 8-bit moments 163 us (0.77 GB, 4.7 TB/s; VALU is
+// not far behind) and 32 us for the norm before it (96 MB, 3.0 TB/s).
 #include "common.h"
 #include "../../include/geomae_hip.h"
 #include <math.h>
