@@ -1105,7 +1105,7 @@ def _to_channels_last(x):
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None):
     """act(group_norm(x)) of a channels-last [N, C, *] tensor (x.movedim(1, -1) contiguous: images in
-    torch.channels_last, [N, C] rows), differentiable once.  x float32 / bfloat16 / float16; weight, bias [C] of one dtype, or
+    torch.channels_last, [N, C] rows), differentiable once, in reverse mode, and not traceable.  x float32 / bfloat16 / float16; weight, bias [C] of one dtype, or
     None; activation None, "relu", "silu" or "gelu" (erf).  y has x's dtype and layout; statistics and sums are fp64 / fp32.
     At most 1024 groups and 2^22 channels.  A backward pass can be captured if no graph of eager work on the default stream holds
     the same leaves (it is refused then)."""
